@@ -365,6 +365,14 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// What is left of (lo, hi) once they have been rounded to the 16-bit pair `rounded`, rounded itself: the pair and
+// the rest together hold about twice the bits.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t rounded) {
+  const T* r = reinterpret_cast<const T*>(&rounded);
+  return pack2<T>(lo - static_cast<float>(r[0]), hi - static_cast<float>(r[1]));
+}
+
 // Packed product of two 16-bit pairs. The exact product of two 16-bit floats fits fp32, so the
 // packed instruction rounds once, exactly like an fp32 multiply followed by a cast.
 template <typename T>

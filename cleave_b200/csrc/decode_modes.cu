@@ -1,0 +1,93 @@
+// Decode attention over a sliding window with sinks, and decode that accumulates attention weights: entry points
+// over the modes of the kernel in decode_attn.cuh, and the kernel that turns kept scores into weights.
+
+#include "decode_attn.cuh"
+
+namespace cb200 {
+namespace {
+
+// weight_sums[b, h, j] += sum over the kv head's query heads g of 2^(x_gj - lse_g), x the score of the decode kernel in
+// log2 units: the softmax weight that key j had in this step. One thread per four keys of a (request, kv head) and
+// one pass over its score rows; a sum has one owner and its heads are added in their order, so the result does not
+// depend on the launch. Bound by the stream of scores (written a moment ago, partly still in L2) and sums.
+constexpr int kSumThreads = 256;
+
+__global__ void __launch_bounds__(kSumThreads) weight_sum_kernel(const DecodeParams p, float* __restrict__ sums) {
+  pdl_wait();
+  const int pair = blockIdx.y, b = pair / p.hkv;
+  const int n = min(item_valid_len(p, b), p.raw_len);
+  const int j = (blockIdx.x * kSumThreads + threadIdx.x) * 4;
+  if (j >= n) return;
+  const size_t row = static_cast<size_t>(pair) * p.rows;
+  const float* x = p.raw + row * p.raw_pitch + j;
+  const float* lse = p.lse + row;
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int g = 0; g < p.rows; ++g) {
+    const float4 v = *reinterpret_cast<const float4*>(x + g * p.raw_pitch);  // pitch and start: multiples of 4
+    const float l = __ldg(lse + g);
+    w[0] += exp2f(v.x - l);
+    w[1] += exp2f(v.y - l);
+    w[2] += exp2f(v.z - l);
+    w[3] += exp2f(v.w - l);
+  }
+  float* dst = sums + static_cast<size_t>(pair) * p.raw_len + j;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (j + i < n) dst[i] += w[i];
+}
+
+// floats between the score rows of two query heads: whole 32-byte runs
+long long raw_pitch(int max_len) { return (static_cast<long long>(max_len) + 7) / 8 * 8; }
+
+}  // namespace
+}  // namespace cb200
+
+extern "C" int cb200_attn_decode_window(const cb200_attn_decode_args* a, int window, int sinks, void* stream) {
+  using namespace cb200;
+  if (!a || !a->kv_indptr || window <= 0 || sinks < 0) return CB200_ERR_BAD_ARG;
+  if (a->q_rows > 1) return CB200_ERR_UNSUPPORTED;  // the window is that of one query, the request's last token
+  DecodeSetup s;
+  const int rc = plan_decode(a, &s, true);
+  if (rc != CB200_OK) return rc;
+  s.p.window = window;
+  s.p.sinks = sinks;
+  return launch_decode_mode<kWindow>(s, a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t cb200_attn_decode_weights_scratch_bytes(const cb200_attn_decode_args* a, int max_len) {
+  if (!a || a->batch <= 0 || a->num_qo_heads <= 0 || max_len <= 0) return 0;
+  return static_cast<size_t>(a->batch) * a->num_qo_heads * cb200::raw_pitch(max_len) * sizeof(float);
+}
+
+extern "C" int cb200_attn_decode_weights(const cb200_attn_decode_args* a, float* weight_sums, int max_len, void* scratch,
+                                         size_t scratch_bytes, void* stream) {
+  using namespace cb200;
+  if (!a || !a->kv_indptr || !a->lse || !weight_sums || max_len <= 0) return CB200_ERR_BAD_ARG;
+  if (a->q_rows > 1) return CB200_ERR_UNSUPPORTED;
+  DecodeSetup s;
+  const int rc = plan_decode(a, &s, true);
+  if (rc != CB200_OK) return rc;
+  const long long pairs = static_cast<long long>(a->batch) * a->num_kv_heads;
+  if (pairs > 65535) return CB200_ERR_UNSUPPORTED;
+  if (!scratch || scratch_bytes < cb200_attn_decode_weights_scratch_bytes(a, max_len)) return CB200_ERR_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(scratch) & 31) || (reinterpret_cast<uintptr_t>(weight_sums) & 15)) return CB200_ERR_ALIGNMENT;
+  s.p.raw = static_cast<float*>(scratch);
+  s.p.raw_len = max_len;
+  s.p.raw_pitch = raw_pitch(max_len);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int done = launch_decode_mode<kWeights>(s, a, st);
+  if (done != CB200_OK) return done;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((max_len + 4LL * kSumThreads - 1) / (4 * kSumThreads)), static_cast<unsigned>(pairs), 1);
+  cfg.blockDim = dim3(kSumThreads, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, weight_sum_kernel, s.p, weight_sums));
+  CB200_CUDA_TRY(cudaGetLastError());
+  return CB200_OK;
+}

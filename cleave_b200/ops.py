@@ -143,6 +143,100 @@ def gqa_paged_decode(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_le
     return out, lse
 
 
+def _one_device(**tensors) -> None:
+    """Refuses tensors that are not all on the device of the first one."""
+    first, where = None, None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if first is None:
+            first, where = name, t.device
+        elif t.device != where:
+            raise ValueError(f"{name} must be on {first}'s device ({where}, not {t.device})")
+
+
+def _launch_workspace(kind: str, nbytes: int, device) -> torch.Tensor:
+    """:func:`workspace`, except while the stream is being captured: two graphs that were captured on one stream may be
+    replayed beside each other, so each call in a graph gets a workspace of its own from the graph's pool, which the
+    graph zero-fills in front of the launch."""
+    if not torch.cuda.is_current_stream_capturing():
+        return workspace(kind, nbytes, device)
+    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+    _lib.check(_lib.lib().cb200_workspace_reset(ws.data_ptr(), ws.numel(), _stream()))
+    return ws
+
+
+def _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, out, lse, max_ctas):
+    """Outputs, checked arguments and workspace of the paged decode variants, on the current device: (out, lse, args,
+    workspace); the caller keeps the workspace alive until it has launched."""
+    if out is None:
+        out = torch.empty_like(q)
+    if lse is None:
+        lse = torch.empty(tuple(q.shape[:2]), dtype=torch.float32, device=q.device)
+    _one_device(q=q, k_cache=k_cache, v_cache=v_cache, kv_indptr=kv_indptr, kv_indices=kv_indices,
+                kv_last_page_len=kv_last_page_len)
+    a = _paged_decode_args(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, out, lse, max_ctas)
+    need = _lib.lib().cb200_attn_decode_workspace_bytes(C.byref(a))
+    if need == 0:
+        _lib.check(_lib.lib().cb200_attn_decode(C.byref(a), _stream()))  # raises the real status
+    ws = _launch_workspace("attn_decode", need, q.device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    return out, lse, a, ws
+
+
+def _window_args(window, sinks):
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
+    limit = 2 ** 31 - 1  # lengths are 32-bit counts: a larger window or number of sinks means all tokens
+    return min(window, limit), min(sinks, limit)
+
+
+def gqa_paged_decode_window(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, window, sinks=0, *,
+                            out=None, lse=None, max_ctas=0):
+    """:func:`gqa_paged_decode` over a sliding window with sinks: of a request's ``n`` tokens the last ``window`` take part
+    and the first ``sinks``. Only the tiles of the cache that hold such a token are read; pages that hold none may have
+    been given away. Returns ``(out, lse)``, ``lse`` base 2 over the tokens that take part; a request without tokens
+    gives 0 / -inf."""
+    window, sinks = _window_args(window, sinks)
+    if _cuda(q, "q").device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return gqa_paged_decode_window(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, window,
+                                           sinks, out=out, lse=lse, max_ctas=max_ctas)
+    out, lse, a, ws = _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, out, lse,
+                                          max_ctas)
+    _lib.check(_lib.lib().cb200_attn_decode_window(C.byref(a), window, sinks, _stream()))
+    return out, lse
+
+
+def gqa_paged_decode_weights(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, weight_sums, *,
+                             out=None, lse=None, max_ctas=0):
+    """:func:`gqa_paged_decode` that also accumulates how much every key has weighed: ``weight_sums[b, h, j]`` grows by the
+    softmax weights of key ``j`` of request ``b``, summed over the query heads of kv head ``h``. ``weight_sums``
+    (batch, HKV, max_len) is a contiguous fp32 tensor, updated in place; entries behind a request's last token stay as
+    they are, and tokens from ``max_len`` on are attended but not recorded. Nothing is added with atomics: the sums are
+    the same bits in every run, and requests may share pages. The scores of the step (4 bytes for every query head and
+    each of ``max_len`` tokens) are kept in scratch memory for the duration of the call. Returns ``(out, lse)``;
+    :func:`kv_cache_evict` reads the sums."""
+    if _cuda(q, "q").device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return gqa_paged_decode_weights(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale,
+                                            weight_sums, out=out, lse=lse, max_ctas=max_ctas)
+    _one_device(q=q, weight_sums=weight_sums)
+    out, lse, a, ws = _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, out, lse,
+                                          max_ctas)
+    if _cuda(weight_sums, "weight_sums").dtype != torch.float32:
+        raise TypeError("weight_sums must be float32")
+    if weight_sums.dim() != 3 or tuple(weight_sums.shape[:2]) != (q.shape[0], k_cache.shape[2]):
+        raise ValueError("weight_sums must be (batch, HKV, max_len)")
+    max_len = weight_sums.shape[2]
+    scratch = torch.empty(_lib.lib().cb200_attn_decode_weights_scratch_bytes(C.byref(a), max_len), dtype=torch.uint8,
+                          device=q.device)
+    _lib.check(_lib.lib().cb200_attn_decode_weights(C.byref(a), weight_sums.data_ptr(), max_len, scratch.data_ptr(),
+                                                    scratch.numel(), _stream()))
+    return out, lse
+
+
 def attention_decode(q, k, v, sm_scale=None, *, out=None, lse=None, max_ctas=0):
     """Static decode attention over contiguous caches. ``q`` (HQ, SQ, D) with a small SQ;
     ``k``, ``v`` (HKV, SKV, D); query head h reads kv head h // (HQ/HKV)

@@ -123,6 +123,27 @@ size_t cb200_attn_decode_workspace_bytes(const cb200_attn_decode_args* a);
 int cb200_attn_decode(const cb200_attn_decode_args* a, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Decode attention over a sliding window with sinks (paged caches): token j of a request with n tokens takes part when
+ * j >= n - window or j < sinks; window >= 1, sinks >= 0. Other tokens are not read, except that a tile of the cache
+ * which holds both kinds may be: what their rows hold does not matter, and pages that hold none of the tokens that
+ * take part may have been given to other requests. Arguments, workspace, `out` and `lse` otherwise as for
+ * cb200_attn_decode. No counterpart in the reference.
+ * ---------------------------------------------------------------------------------------- */
+int cb200_attn_decode_window(const cb200_attn_decode_args* a, int window, int sinks, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Decode attention (paged caches) that also accumulates what every key has weighed:
+ *   weight_sums[b, h, j] += sum over the query heads of kv head h of softmax weight j     (fp32)
+ * weight_sums is (batch, num_kv_heads, max_len), contiguous, 16-byte aligned, updated in place; entries behind a
+ * request's last token are left as they are, tokens from max_len on are attended but not recorded. Requests may share
+ * pages. `lse` must not be NULL. `scratch` (cb200_attn_decode_weights_scratch_bytes, 32-byte aligned, any contents) holds
+ * the scores between the two kernels. batch * num_kv_heads <= 65535. No counterpart in the reference.
+ * ---------------------------------------------------------------------------------------- */
+size_t cb200_attn_decode_weights_scratch_bytes(const cb200_attn_decode_args* a, int max_len);
+int cb200_attn_decode_weights(const cb200_attn_decode_args* a, float* weight_sums, int max_len, void* scratch,
+                              size_t scratch_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Fused dense contractions on the tcgen05 tensor cores. X is (m, k) row-major, W (and W1) are
  * (k, n) row-major, Y is (m, n) row-major; k and n must be multiples of 8.
  *   CB200_GEMM_MATMUL   Y = X @ W
