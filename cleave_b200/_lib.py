@@ -38,6 +38,17 @@ class AttnDecodeArgs(C.Structure):
     ]
 
 
+class KvEvictArgs(C.Structure):
+    _fields_ = [
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("weight_sums", C.c_void_p), ("kv_indptr", C.c_void_p),
+        ("kv_indices", C.c_void_p), ("kv_last_page_len", C.c_void_p), ("dst_indptr", C.c_void_p),
+        ("dst_indices", C.c_void_p), ("kept", C.c_void_p), ("kept_sums", C.c_void_p), ("dst_last_page_len", C.c_void_p),
+        ("batch", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32),
+        ("num_pages", C.c_int32), ("num_kv_indices", C.c_int32), ("num_dst_indices", C.c_int32), ("max_len", C.c_int32),
+        ("budget", C.c_int32), ("sinks", C.c_int32), ("recent", C.c_int32),
+    ]
+
+
 class GemmArgs(C.Structure):
     _fields_ = [
         ("x", C.c_void_p), ("w", C.c_void_p), ("w1", C.c_void_p), ("gamma", C.c_void_p), ("y", C.c_void_p),
@@ -187,6 +198,8 @@ def lib() -> C.CDLL:
         L.cb200_attn_decode_weights.restype = C.c_int
         L.cb200_attn_decode_weights.argtypes = [C.POINTER(AttnDecodeArgs), C.c_void_p, C.c_int, C.c_void_p, C.c_size_t,
                                                 C.c_void_p]
+        L.cb200_kv_evict.restype = C.c_int
+        L.cb200_kv_evict.argtypes = [C.POINTER(KvEvictArgs), C.c_void_p]
         L.cb200_workspace_reset.restype = C.c_int
         L.cb200_workspace_reset.argtypes = [C.c_void_p, C.c_size_t, C.c_void_p]
         L.cb200_gemm_workspace_bytes.restype = C.c_size_t

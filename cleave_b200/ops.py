@@ -237,6 +237,65 @@ def gqa_paged_decode_weights(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last
     return out, lse
 
 
+def kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last_page_len, dst_indptr, dst_indices, *, budget,
+                   sinks=0, recent=0):
+    """Shortens the requests of a paged cache to at most ``budget`` tokens each: per kv head the first ``sinks`` tokens, the
+    last ``recent`` and, of the others, those with the largest ``weight_sums`` (the accumulators of
+    :func:`gqa_paged_decode_weights`; equal sums: the lower index; NaN counts as the largest value) are copied in their
+    order into the pages that ``dst_indptr`` / ``dst_indices`` list. Caches (num_pages, page_size, HKV, D);
+    ``weight_sums`` (batch, HKV, max_len) fp32; ``kv_indptr`` and ``dst_indptr`` (batch + 1) int32 in pages. Give a
+    request of ``n`` tokens ``ceil(min(n, budget) / page_size)`` destination pages (with fewer, fewer tokens stay).
+    Source pages are only read and may be shared; destination pages must be pages of the same pool that are neither
+    source pages of this call nor used twice. Returns ``(kept, sums, last_page_len)``: the kept indices (batch, HKV,
+    budget) int32, ascending, then -1; new accumulators (batch, HKV, max_len) that hold the kept tokens' sums, then 0; and
+    (batch) int32, which with the destination tables is the shortened requests' page table."""
+    if _cuda(k_cache, "k_cache").device.index != torch.cuda.current_device():
+        with torch.cuda.device(k_cache.device):
+            return kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last_page_len, dst_indptr, dst_indices,
+                                  budget=budget, sinks=sinks, recent=recent)
+    _cuda(v_cache, "v_cache"), _cuda(weight_sums, "weight_sums")
+    _one_device(k_cache=k_cache, v_cache=v_cache, weight_sums=weight_sums, kv_indptr=kv_indptr, kv_indices=kv_indices,
+                kv_last_page_len=kv_last_page_len, dst_indptr=dst_indptr, dst_indices=dst_indices)
+    budget, sinks, recent = int(budget), int(sinks), int(recent)
+    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError(f"budget must be at least 1 and at least sinks + recent, got {budget}, {sinks} and {recent}")
+    _dtype_code(k_cache)
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        raise ValueError("the caches must be (num_pages, page_size, HKV, D), of one storage dtype")
+    num_pages, page_size, hkv, d = k_cache.shape
+    if weight_sums.dtype != torch.float32:
+        raise TypeError("weight_sums must be float32")
+    if weight_sums.dim() != 3 or weight_sums.shape[1] != hkv:
+        raise ValueError("weight_sums must be (batch, HKV, max_len)")
+    batch, _, max_len = weight_sums.shape
+    tables = {"kv_indptr": kv_indptr, "kv_indices": kv_indices, "dst_indptr": dst_indptr, "dst_indices": dst_indices}
+    if page_size != 1 and kv_last_page_len is None:
+        raise TypeError("missing input 'kv_last_page_len'")
+    if kv_last_page_len is not None:
+        tables["kv_last_page_len"] = kv_last_page_len
+    for name, t in tables.items():
+        if _cuda(t, name).dtype != torch.int32:
+            raise TypeError(f"{name} must be int32")
+    if kv_indptr.numel() != batch + 1 or dst_indptr.numel() != batch + 1:
+        raise ValueError("kv_indptr and dst_indptr must have batch + 1 entries")
+    if kv_last_page_len is not None and kv_last_page_len.numel() != batch:
+        raise ValueError("kv_last_page_len must hold batch values")
+    kept = torch.empty((batch, hkv, budget), dtype=torch.int32, device=k_cache.device)
+    sums = torch.empty_like(weight_sums)
+    last = torch.empty(batch, dtype=torch.int32, device=k_cache.device)
+    a = _lib.KvEvictArgs()
+    a.k_cache, a.v_cache, a.weight_sums = k_cache.data_ptr(), v_cache.data_ptr(), weight_sums.data_ptr()
+    a.kv_indptr, a.kv_indices = kv_indptr.data_ptr(), kv_indices.data_ptr()
+    a.kv_last_page_len = None if kv_last_page_len is None else kv_last_page_len.data_ptr()
+    a.dst_indptr, a.dst_indices = dst_indptr.data_ptr(), dst_indices.data_ptr()
+    a.kept, a.kept_sums, a.dst_last_page_len = kept.data_ptr(), sums.data_ptr(), last.data_ptr()
+    a.batch, a.num_kv_heads, a.head_dim, a.page_size, a.num_pages = batch, hkv, d, page_size, num_pages
+    a.num_kv_indices, a.num_dst_indices, a.max_len = kv_indices.numel(), dst_indices.numel(), max_len
+    a.budget, a.sinks, a.recent = budget, sinks, recent
+    _lib.check(_lib.lib().cb200_kv_evict(C.byref(a), _stream()))
+    return kept, sums, last
+
+
 def attention_decode(q, k, v, sm_scale=None, *, out=None, lse=None, max_ctas=0):
     """Static decode attention over contiguous caches. ``q`` (HQ, SQ, D) with a small SQ;
     ``k``, ``v`` (HKV, SKV, D); query head h reads kv head h // (HQ/HKV)

@@ -144,6 +144,40 @@ int cb200_attn_decode_weights(const cb200_attn_decode_args* a, float* weight_sum
                               size_t scratch_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Eviction from a paged cache by accumulated attention weight (the sums cb200_attn_decode_weights keeps). Per (request, kv
+ * head) with n tokens, B = min(n, budget, room in its destination pages) tokens stay: the first min(sinks, B), the last
+ * min(recent, B - those), and of the tokens between them the ones with the largest weight sums (equal sums: the lower
+ * index; NaN counts as the largest value; tokens from max_len on count as 0). Their rows of K and V are copied, in their
+ * order, to the slots 0 .. B - 1 of the request's destination pages, which have the layout of the source pages and
+ * belong to the same pool. Source pages are only read, so requests may share them; the destination pages must be
+ * disjoint from one another and from all source pages of the call. The table that dst_indptr / dst_indices /
+ * dst_last_page_len form is that of the shortened requests where dst_indptr gives each of them ceil(B / page_size) pages.
+ *   kept              (batch, num_kv_heads, budget): the indices that stay, ascending, then -1
+ *   kept_sums         (batch, num_kv_heads, max_len): their sums, then 0; must not overlap weight_sums
+ *   dst_last_page_len (batch): tokens in the last destination page, 0 for B = 0
+ * sinks + recent <= budget, head_dim a multiple of 8, 16-bit elements of either type, batch <= 65535. Page tables are not
+ * trusted: ranges are clipped to the tables, source pages to the pool, and rows whose destination page does not exist
+ * are not written. Two kernels, no workspace. No counterpart in the reference.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct {
+  void* k_cache;                   /* (num_pages, page_size, num_kv_heads, head_dim) */
+  void* v_cache;
+  const float* weight_sums;        /* (batch, num_kv_heads, max_len) */
+  const int32_t* kv_indptr;        /* (batch + 1) */
+  const int32_t* kv_indices;       /* (num_kv_indices) */
+  const int32_t* kv_last_page_len; /* (batch); may be NULL when page_size == 1 */
+  const int32_t* dst_indptr;       /* (batch + 1) */
+  const int32_t* dst_indices;      /* (num_dst_indices) */
+  int32_t* kept;
+  float* kept_sums;
+  int32_t* dst_last_page_len;
+  int32_t batch, num_kv_heads, head_dim, page_size, num_pages, num_kv_indices, num_dst_indices;
+  int32_t max_len, budget, sinks, recent;
+} cb200_kv_evict_args;
+
+int cb200_kv_evict(const cb200_kv_evict_args* a, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Fused dense contractions on the tcgen05 tensor cores. X is (m, k) row-major, W (and W1) are
  * (k, n) row-major, Y is (m, n) row-major; k and n must be multiples of 8.
  *   CB200_GEMM_MATMUL   Y = X @ W
