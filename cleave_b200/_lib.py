@@ -198,6 +198,11 @@ def lib() -> C.CDLL:
         L.cb200_attn_decode_weights.restype = C.c_int
         L.cb200_attn_decode_weights.argtypes = [C.POINTER(AttnDecodeArgs), C.c_void_p, C.c_int, C.c_void_p, C.c_size_t,
                                                 C.c_void_p]
+        L.cb200_attn_decode_shared_prefix_scratch_bytes.restype = C.c_size_t
+        L.cb200_attn_decode_shared_prefix_scratch_bytes.argtypes = [C.POINTER(AttnDecodeArgs), C.c_int]
+        L.cb200_attn_decode_shared_prefix.restype = C.c_int
+        L.cb200_attn_decode_shared_prefix.argtypes = [C.POINTER(AttnDecodeArgs), C.c_void_p, C.c_int, C.c_int, C.c_void_p,
+                                                      C.c_size_t, C.c_void_p]
         L.cb200_kv_evict.restype = C.c_int
         L.cb200_kv_evict.argtypes = [C.POINTER(KvEvictArgs), C.c_void_p]
         L.cb200_workspace_reset.restype = C.c_int

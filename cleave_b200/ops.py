@@ -237,6 +237,33 @@ def gqa_paged_decode_weights(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last
     return out, lse
 
 
+def gqa_paged_decode_shared_prefix(q, k_cache, v_cache, prefix_indices, prefix_len, kv_indptr, kv_indices, kv_last_page_len,
+                                   sm_scale, *, out=None, lse=None, max_ctas=0):
+    """:func:`gqa_paged_decode` for a batch whose requests share a prefix: every request attends the ``prefix_len`` tokens of
+    the pages ``prefix_indices`` (int32), then its own tokens, which ``kv_indptr`` / ``kv_indices`` / ``kv_last_page_len``
+    describe as usual (a request may have none). The prefix's rows are read once for the batch, not once per request.
+    ``prefix_len`` is a number; only the first ``ceil(prefix_len / page_size)`` entries of ``prefix_indices`` are used. At
+    most 128 query heads per kv head. Returns ``(out, lse)`` over both parts, ``lse`` base 2."""
+    if _cuda(q, "q").device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return gqa_paged_decode_shared_prefix(q, k_cache, v_cache, prefix_indices, prefix_len, kv_indptr, kv_indices,
+                                                  kv_last_page_len, sm_scale, out=out, lse=lse, max_ctas=max_ctas)
+    prefix_len = int(prefix_len)
+    _one_device(q=q, prefix_indices=_cuda(prefix_indices, "prefix_indices"))
+    out, lse, a, ws = _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, out, lse,
+                                          max_ctas)
+    if prefix_indices.dtype != torch.int32:
+        raise TypeError("prefix_indices must be int32")
+    if prefix_len < 0 or prefix_len > prefix_indices.numel() * k_cache.shape[1]:
+        raise ValueError(f"prefix_len must be between 0 and the {prefix_indices.numel()} pages of prefix_indices, got {prefix_len}")
+    L = _lib.lib()
+    need = L.cb200_attn_decode_shared_prefix_scratch_bytes(C.byref(a), prefix_len)
+    scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _lib.check(L.cb200_attn_decode_shared_prefix(C.byref(a), prefix_indices.data_ptr(), prefix_indices.numel(), prefix_len,
+                                                 scratch.data_ptr(), need, _stream()))
+    return out, lse
+
+
 def kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last_page_len, dst_indptr, dst_indices, *, budget,
                    sinks=0, recent=0):
     """Shortens the requests of a paged cache to at most ``budget`` tokens each: per kv head the first ``sinks`` tokens, the

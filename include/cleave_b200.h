@@ -144,6 +144,19 @@ int cb200_attn_decode_weights(const cb200_attn_decode_args* a, float* weight_sum
                               size_t scratch_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Decode attention (paged caches) of a batch that shares a prefix: request b attends the prefix_len tokens of the pages
+ * prefix_indices[0 .. ceil(prefix_len / page_size)) and then its own tokens, those of `a`'s page table, which may be none.
+ * The prefix's keys and values are read once for the batch, on the tcgen05 tensor cores. `out` and `lse` cover both
+ * parts; a request with neither gives 0 / -inf. prefix_len = 0 is plain decode (prefix_indices and scratch may then be
+ * NULL). num_qo_heads / num_kv_heads <= 128, prefix_len <= 2^30. `scratch`
+ * (cb200_attn_decode_shared_prefix_scratch_bytes, 16-byte aligned, any contents; 0 bytes for prefix_len = 0) holds fp32
+ * partials between the two kernels; the workspace is that of cb200_attn_decode. No counterpart in the reference.
+ * ---------------------------------------------------------------------------------------- */
+size_t cb200_attn_decode_shared_prefix_scratch_bytes(const cb200_attn_decode_args* a, int prefix_len);
+int cb200_attn_decode_shared_prefix(const cb200_attn_decode_args* a, const int32_t* prefix_indices, int num_prefix_indices,
+                                    int prefix_len, void* scratch, size_t scratch_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Eviction from a paged cache by accumulated attention weight (the sums cb200_attn_decode_weights keeps). Per (request, kv
  * head) with n tokens, B = min(n, budget, room in its destination pages) tokens stay: the first min(sinks, B), the last
  * min(recent, B - those), and of the tokens between them the ones with the largest weight sums (equal sums: the lower
