@@ -203,6 +203,8 @@ def lib() -> C.CDLL:
         L.cb200_attn_decode_shared_prefix.restype = C.c_int
         L.cb200_attn_decode_shared_prefix.argtypes = [C.POINTER(AttnDecodeArgs), C.c_void_p, C.c_int, C.c_int, C.c_void_p,
                                                       C.c_size_t, C.c_void_p]
+        L.cb200_attn_prefill_ragged_window.restype = C.c_int
+        L.cb200_attn_prefill_ragged_window.argtypes = [C.POINTER(AttnPrefillRaggedArgs), C.c_int, C.c_int, C.c_int, C.c_void_p]
         L.cb200_kv_evict.restype = C.c_int
         L.cb200_kv_evict.argtypes = [C.POINTER(KvEvictArgs), C.c_void_p]
         L.cb200_workspace_reset.restype = C.c_int

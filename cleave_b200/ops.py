@@ -515,6 +515,86 @@ def gqa_paged_prefill(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_
                               lse=lse, kv_indices=_cuda(kv_indices, "kv_indices"))
 
 
+def _prefill_window(q, k, v, qo_indptr, kv_indptr, kv_indices, sm_scale, window, sinks, out, lse):
+    total_q, hq, d = q.shape
+    total_kv, hkv, _ = k.shape
+    a = _lib.AttnPrefillRaggedArgs()
+    fill = (1 if out is None else 0) | (2 if lse is None else 0)
+    if out is None:
+        out = torch.empty_like(q)
+    if lse is None:
+        lse = torch.empty((total_q, hq), dtype=torch.float32, device=q.device)
+    if _cuda(out, "out").shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError("out must have q's shape, dtype and device")
+    if tuple(_cuda(lse, "lse").shape) != (total_q, hq) or lse.dtype != torch.float32 or lse.device != q.device:
+        raise ValueError("lse must be (total_q, HQ) float32 on q's device")
+    a.q, a.k, a.v, a.out, a.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr()
+    a.qo_indptr, a.kv_indptr = qo_indptr.data_ptr(), kv_indptr.data_ptr()
+    if kv_indices is not None:
+        a.kv_indices, a.num_kv_indices = kv_indices.data_ptr(), kv_indices.numel()
+    a.batch, a.total_q, a.total_kv = qo_indptr.numel() - 1, total_q, total_kv
+    a.num_qo_heads, a.num_kv_heads, a.head_dim = hq, hkv, d
+    a.dtype, a.causal, a.sm_scale = _dtype_code(q), 1, float(sm_scale)
+    L = _lib.lib()
+    need = L.cb200_attn_prefill_ragged_workspace_bytes(C.byref(a))
+    if need == 0:
+        _lib.check(L.cb200_attn_prefill_ragged_window(C.byref(a), window, sinks, fill, _stream()))  # raises the real status
+    ws = _launch_workspace("attn_prefill", need, q.device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _lib.check(L.cb200_attn_prefill_ragged_window(C.byref(a), window, sinks, fill, _stream()))
+    return out, lse
+
+
+def gqa_ragged_prefill_window(q, k, v, qo_indptr, kv_indptr, sm_scale, window, sinks=0, *, out=None, lse=None):
+    """:func:`gqa_ragged_prefill` over a sliding window with sinks: the query at position ``p`` of its request (counted from
+    the request's end, as the causal mask does) sees key ``j <= p`` when ``j > p - window`` or ``j < sinks``. Always
+    causal. Returns ``(out, lse)``; rows that see no key are 0 / -inf, and so are rows that belong to no request where
+    ``out`` / ``lse`` are allocated here (in tensors of the caller they stay as they are)."""
+    window, sinks = _window_args(window, sinks)
+    if _cuda(q, "q").device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return gqa_ragged_prefill_window(q, k, v, qo_indptr, kv_indptr, sm_scale, window, sinks, out=out, lse=lse)
+    _cuda(k, "k"), _cuda(v, "v")
+    if q.dim() != 3 or k.dim() != 3 or k.shape[2] != q.shape[2] or v.shape != k.shape or k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError("shapes: q (total_q,HQ,D), k/v (total_kv,HKV,D), HQ a multiple of HKV")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must share one storage dtype")
+    if _cuda(qo_indptr, "qo_indptr").dtype != torch.int32 or _cuda(kv_indptr, "kv_indptr").dtype != torch.int32:
+        raise TypeError("qo_indptr / kv_indptr must be int32")
+    if qo_indptr.numel() < 2 or qo_indptr.numel() != kv_indptr.numel():
+        raise ValueError("qo_indptr and kv_indptr must both hold batch + 1 entries")
+    _one_device(q=q, k=k, v=v, qo_indptr=qo_indptr, kv_indptr=kv_indptr)
+    return _prefill_window(q, k, v, qo_indptr, kv_indptr, None, sm_scale, window, sinks, out, lse)
+
+
+def gqa_paged_prefill_window(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_scale, window, sinks=0, *, out=None,
+                             lse=None):
+    """:func:`gqa_paged_prefill` over a sliding window with sinks (see :func:`gqa_ragged_prefill_window`): caches
+    (num_pages, 1, HKV, D), one token per page. Pages of tokens that no query of the call sees may have been given
+    away."""
+    window, sinks = _window_args(window, sinks)
+    if _cuda(q, "q").device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return gqa_paged_prefill_window(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_scale, window, sinks, out=out,
+                                            lse=lse)
+    _cuda(k_cache, "k_cache"), _cuda(v_cache, "v_cache")
+    if k_cache.dim() != 4 or k_cache.shape[1] != 1 or v_cache.shape != k_cache.shape:
+        raise ValueError("caches: (num_pages, 1, HKV, D), one token per page")
+    if q.dim() != 3 or k_cache.shape[3] != q.shape[2] or k_cache.shape[2] == 0 or q.shape[1] % k_cache.shape[2]:
+        raise ValueError("shapes: q (total_q,HQ,D), caches (num_pages,1,HKV,D), HQ a multiple of HKV")
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise TypeError("q and the caches must share one storage dtype")
+    for name, t in (("qo_indptr", qo_indptr), ("kv_indptr", kv_indptr), ("kv_indices", kv_indices)):
+        if _cuda(t, name).dtype != torch.int32:
+            raise TypeError(f"{name} must be int32")
+    if kv_indices.numel() == 0:
+        raise ValueError("kv_indices must hold at least one page")
+    if qo_indptr.numel() < 2 or qo_indptr.numel() != kv_indptr.numel():
+        raise ValueError("qo_indptr and kv_indptr must both hold batch + 1 entries")
+    _one_device(q=q, k_cache=k_cache, v_cache=v_cache, qo_indptr=qo_indptr, kv_indptr=kv_indptr, kv_indices=kv_indices)
+    return _prefill_window(q, k_cache[:, 0], v_cache[:, 0], qo_indptr, kv_indptr, kv_indices, sm_scale, window, sinks, out, lse)
+
+
 def gqa_paged_decode_static_scratch(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale,
                                     *, out, lse, max_ctas=0):
     """Paged decode for hosts that may not allocate device memory (a server that gave this

@@ -400,6 +400,15 @@ typedef struct {
 size_t cb200_attn_prefill_ragged_workspace_bytes(const cb200_attn_prefill_ragged_args* a);
 int cb200_attn_prefill_ragged(const cb200_attn_prefill_ragged_args* a, void* stream);
 
+/* Ragged or paged causal prefill over a sliding window with sinks: the query at position p of its request (the causal
+ * mask's p = row + kv_len - q_len) sees key j <= p when j > p - window or j < sinks; window >= 1, sinks >= 0. Always
+ * causal (`a->causal` is not looked at). Keys that no query of the call sees are not read or add nothing, whatever their
+ * rows hold; page ids of such keys may name pages that belong to others. fill, bit 0: rows of `out` that belong to no
+ * request (in front of the first or behind the last) become 0, bit 1: those of `lse` become -inf; without the bit they
+ * stay as they are. Arguments, workspace
+ * (cb200_attn_prefill_ragged_workspace_bytes) and results otherwise as above. No counterpart in the reference. */
+int cb200_attn_prefill_ragged_window(const cb200_attn_prefill_ragged_args* a, int window, int sinks, int fill, void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * O = (Q K^T) V without softmax or scale; q (num_qo_heads, q_len, head_dim), k / v (num_kv_heads, kv_len,
  * head_dim), query head h uses kv head h / (HQ / HKV); head_dim 64 or 128. Replaces the fused kernel of
