@@ -5,8 +5,8 @@
 // sums; equal sums go to the lower index, NaN counts as the largest value. The kept rows of K and V are copied, in
 // their order, into the destination pages, and their sums with them.
 //
-// Two kernels. evict_select_kernel (one CTA per (request, kv head)) finds the smallest kept sum by a radix select over
-// the sums' bits and writes the kept indices in order. evict_copy_kernel moves the rows: it has no dependence between
+// Two kernels. evict_select_kernel (one CTA per (request, kv head)) finds the smallest kept sum with two or three
+// histograms over the sums, which it holds in registers, and writes the kept indices in order. evict_copy_kernel moves the rows: it has no dependence between
 // its CTAs (source and destination pages are disjoint), so it is a plain gather of 2 D-byte rows that is bound by the
 // memory's bandwidth, which is nearly all of the operator's time where the cache is large.
 
@@ -16,8 +16,9 @@ namespace cb200 {
 namespace {
 
 constexpr int kSelThreads = 512;
+constexpr int kBinBits = 11, kBins = 1 << kBinBits;  // four bins a thread
+constexpr int kKeysMost = 64;   // sums a thread of the select kernel holds at most
 constexpr int kCopyThreads = 256;
-constexpr int kCopyRows = 128;  // (token, head) rows of K and of V per CTA
 
 struct EvictParams {
   uint4* k;
@@ -67,10 +68,16 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictParams p) {
-  __shared__ int hist[256];
-  __shared__ int found[2];  // digit, values above it
-  __shared__ int warp_strict[kSelThreads / 32], warp_tie[kSelThreads / 32];
+// KEYS: sums a thread holds in registers (thread t of the CTA: tokens lo + t, lo + t + 512, ...). The sums of a longer
+// range are read again in every step.
+template <int KEYS>
+__global__ void __launch_bounds__(kSelThreads, KEYS <= 16 ? 2 : 1) evict_select_kernel(const EvictParams p) {
+  constexpr int kWarps = kSelThreads / 32;
+  __shared__ __align__(16) int bins[kBins];
+  __shared__ uint32_t range[2][kWarps];
+  __shared__ int warp_sum[kWarps], found[3];  // found: bin, keys in bins above it, keys in it
+  __shared__ uint32_t slab[KEYS * kWarps];  // tokens above the threshold, and those equal to it << 16
+  __shared__ uint32_t slab_all;
   pdl_wait();
   pdl_launch_dependents();
   const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -83,6 +90,13 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
   const int lo = first, hi = r.n - tail;      // the tokens that are ranked: lo <= j < hi
   const int middle = r.keep - first - tail;   // of which this many stay
   auto sum_of = [&](int j) { return j < p.max_len ? __ldg(sums + j) : 0.f; };  // tokens without a record weigh nothing
+  auto key_of = [&](int j) { return j < hi ? order_key(sum_of(j)) : 0u; };     // no sum has the key 0
+  const bool rank = middle > 0 && middle < hi - lo;
+  uint32_t key[KEYS];
+  if (rank) {
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) key[i] = key_of(lo + i * kSelThreads + tid);
+  }
 
   if (h == 0 && tid == 0) p.dst_last[b] = r.keep > 0 ? (r.keep - 1) % p.page_size + 1 : 0;
   auto put = [&](int i, int j) {
@@ -93,88 +107,147 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
   for (int i = tid; i < tail; i += kSelThreads) put(r.keep - tail + i, r.n - tail + i);
   for (int i = r.keep + tid; i < p.budget; i += kSelThreads) kept[i] = -1;
   for (int i = r.keep + tid; i < p.max_len; i += kSelThreads) kept_sums[i] = 0.f;
-  if (middle <= 0) return;
-  if (middle == hi - lo) {
+  if (!rank) {
     for (int i = tid; i < middle; i += kSelThreads) put(lo + i, lo + i);
     return;
   }
 
-  // ---- the key of rank `middle`, eight bits at a time from the top
-  uint32_t prefix = 0;
-  int want = middle;  // its rank among the keys that share the prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+  auto each_key = [&](auto&& f) {  // every ranked key of this thread
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i)
+      if (lo + i * kSelThreads + tid < hi) f(key[i]);
+    for (int j = lo + KEYS * kSelThreads + tid; j < hi; j += kSelThreads) f(key_of(j));
+  };
+  // ---- the key of rank `middle`, by histograms over ranges of keys that shrink by kBins a round. The first range
+  // is that of the keys themselves, not of all 32-bit numbers: sums of attention weights span a few dozen exponents, and
+  // a key is about the logarithm of its sum, so kBins equal steps spread them thinly where fixed digits would
+  // pile them up in a few bins and their counting in a few words of shared memory.
+  uint32_t base = 0xffffffffu, top = 0;
+  each_key([&](uint32_t k) {
+    base = min(base, k);
+    top = max(top, k);
+  });
+  base = __reduce_min_sync(0xffffffffu, base);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) {
+    range[0][warp] = base;
+    range[1][warp] = top;
+  }
+  for (int i = tid; i < kBins; i += kSelThreads) bins[i] = 0;
+  __syncthreads();
+  base = __reduce_min_sync(0xffffffffu, range[0][lane & (kWarps - 1)]);
+  top = __reduce_max_sync(0xffffffffu, range[1][lane & (kWarps - 1)]);
+  int want = middle, ties = 0;  // rank inside the range; in the end: how many of the keys equal to the threshold stay
+  uint32_t threshold;           // keys above it stay
+  while (true) {
+    const int shift = max(32 - __clz(top - base) - kBinBits, 0);
+    each_key([&](uint32_t k) {
+      if (k >= base && k <= top) atomicAdd(&bins[(k - base) >> shift], 1);
+    });
     __syncthreads();
-    for (int j = lo + tid; j < hi; j += kSelThreads) {
-      const uint32_t key = order_key(sum_of(j));
-      if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
+    // a thread's four bins, largest keys first, scanned over the CTA
+    const int4 c = *reinterpret_cast<const int4*>(&bins[kBins - 4 * (tid + 1)]);
+    const int mine = c.x + c.y + c.z + c.w;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    *reinterpret_cast<int4*>(&bins[kBins - 4 * (tid + 1)]) = make_int4(0, 0, 0, 0);  // for the next round
+    int above = incl - mine;
+    for (int w = 0; w < warp; ++w) above += warp_sum[w];
+    if (above < want && want <= above + mine) {
+      int bin = kBins - 1 - 4 * tid, n = c.w;
+      if (above + n < want) { above += n; --bin; n = c.z; }
+      if (above + n < want) { above += n; --bin; n = c.y; }
+      if (above + n < want) { above += n; --bin; n = c.x; }
+      found[0] = bin;
+      found[1] = above;
+      found[2] = n;
+    }
+    __syncthreads();
+    const uint32_t low = base + (static_cast<uint32_t>(found[0]) << shift);
+    want -= found[1];
+    if (found[2] == want) {  // all of the bin stays
+      threshold = low - 1;
+      break;
+    }
+    if (shift == 0) {  // one value, more often than it is wanted
+      threshold = low;
+      ties = want;
+      break;
+    }
+    base = low;
+    top = min(top, low + ((1u << shift) - 1));
+  }
+
+  // ---- keys above the threshold stay, and the first `ties` of those equal to it. Where a kept token goes follows from how
+  // many stay before it: per slab of 512 tokens and warp the counts are taken from ballots, scanned once over all of
+  // them by one warp, and added to the place inside the warp.
+  int done_strict = 0, done_tie = 0;  // before this round of slabs
+  const uint32_t below = (1u << lane) - 1;
+  for (int j0 = lo; j0 < hi; j0 += KEYS * kSelThreads) {
+    if (j0 > lo) {
+#pragma unroll
+      for (int i = 0; i < KEYS; ++i) key[i] = key_of(j0 + i * kSelThreads + tid);
+    }
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      const uint32_t bs = __ballot_sync(0xffffffffu, key[i] > threshold), bt = ties ? __ballot_sync(0xffffffffu, key[i] == threshold) : 0u;
+      if (lane == 0) slab[i * kWarps + warp] = __popc(bs) | __popc(bt) << 16;
     }
     __syncthreads();
     if (warp == 0) {
-      // lane l holds the digits 255 - 8 l .. 248 - 8 l, largest first
-      int mine = 0, c[8];
+      constexpr int kPer = (KEYS * kWarps + 31) / 32;
+      uint32_t mine = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mine += c[i] = hist[255 - 8 * lane - i];
-      int incl = mine;
+      for (int i = 0; i < kPer; ++i) mine += slab[lane * kPer + i];  // at most 512 KEYS <= 32768 per half: no carry
+      uint32_t incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += v;
       }
-      int above = incl - mine;
-      if (above < want && want <= incl) {
+      uint32_t run = incl - mine;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (above < want && want <= above + c[i]) {
-            found[0] = 255 - 8 * lane - i;
-            found[1] = above;
-          }
-          above += c[i];
-        }
+      for (int i = 0; i < kPer; ++i) {
+        const uint32_t t = slab[lane * kPer + i];
+        slab[lane * kPer + i] = run;
+        run += t;
       }
+      if (lane == 31) slab_all = run;
     }
     __syncthreads();
-    prefix = (prefix << 8) | static_cast<uint32_t>(found[0]);
-    want -= found[1];
-  }
-  // keys above `prefix` stay, and the first `want` of those equal to it
-  int done_strict = 0, done_tie = 0;
-  for (int j0 = lo; j0 < hi; j0 += kSelThreads) {
-    const int j = j0 + tid;
-    const uint32_t key = j < hi ? order_key(sum_of(j)) : 0u;
-    const bool strict = j < hi && key > prefix, tie = j < hi && key == prefix;
-    const uint32_t bs = __ballot_sync(0xffffffffu, strict), bt = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) {
-      warp_strict[warp] = __popc(bs);
-      warp_tie[warp] = __popc(bt);
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      const bool strict = key[i] > threshold, tie = ties && key[i] == threshold;
+      const uint32_t bs = __ballot_sync(0xffffffffu, strict), bt = ties ? __ballot_sync(0xffffffffu, tie) : 0u;
+      const uint32_t before = slab[i * kWarps + warp];
+      const int s = done_strict + static_cast<int>(before & 0xffffu) + __popc(bs & below);
+      const int t = done_tie + static_cast<int>(before >> 16) + __popc(bt & below);
+      const int j = j0 + i * kSelThreads + tid;
+      if (strict || (tie && t < ties)) put(lo + s + min(t, ties), j);
     }
-    __syncthreads();
-    int s = done_strict, t = done_tie;
-    for (int w = 0; w < kSelThreads / 32; ++w) {
-      if (w < warp) {
-        s += warp_strict[w];
-        t += warp_tie[w];
-      }
-      done_strict += warp_strict[w];
-      done_tie += warp_tie[w];
-    }
-    const uint32_t below = (1u << lane) - 1;
-    s += __popc(bs & below);
-    t += __popc(bt & below);
-    if (strict || (tie && t < want)) put(lo + s + min(t, want), j);
+    done_strict += slab_all & 0xffffu;
+    done_tie += slab_all >> 16;
     __syncthreads();
   }
 }
 
+// ROWS: (token, head) rows of K and of V per CTA
+template <int ROWS>
 __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const EvictParams p) {
-  __shared__ long long src_off[kCopyRows], dst_off[kCopyRows];  // in 16-byte chunks; dst < 0: no such page
+  __shared__ long long src_off[ROWS], dst_off[ROWS];  // in 16-byte chunks; dst < 0: no such page
   pdl_wait();
   const int b = blockIdx.y;
   const Request r = request_of(p, b);
   const long long rows = static_cast<long long>(r.keep) * p.hkv;  // (token, head), heads innermost
-  const long long r0 = static_cast<long long>(blockIdx.x) * kCopyRows;
+  const long long r0 = static_cast<long long>(blockIdx.x) * ROWS;
   if (r0 >= rows) return;
-  const int here = static_cast<int>(min(static_cast<long long>(kCopyRows), rows - r0));
+  const int here = static_cast<int>(min(static_cast<long long>(ROWS), rows - r0));
   for (int x = threadIdx.x; x < here; x += kCopyThreads) {
     const int i = static_cast<int>((r0 + x) / p.hkv), h = static_cast<int>((r0 + x) % p.hkv);
     const int j = __ldcg(p.kept + (static_cast<size_t>(b) * p.hkv + h) * p.budget + i);
@@ -222,7 +295,10 @@ extern "C" int cb200_kv_evict(const cb200_kv_evict_args* a, void* stream) {
   if (a->head_dim % 8 || a->batch > 65535) return CB200_ERR_UNSUPPORTED;
   // token counts are held in 32 bits
   if (static_cast<long long>(a->num_kv_indices) * a->page_size >= (1LL << 31)) return CB200_ERR_UNSUPPORTED;
-  const long long copy_ctas = (static_cast<long long>(a->budget) * a->num_kv_heads + kCopyRows - 1) / kCopyRows;
+  // Small CTAs where the rows would not give every SM several large ones (one request of 512 tokens and 8 heads).
+  const long long rows = static_cast<long long>(a->budget) * a->num_kv_heads;
+  const int copy_rows = rows * a->batch >= 128LL * 4 * 148 ? 128 : 32;
+  const long long copy_ctas = (rows + copy_rows - 1) / copy_rows;
   if (copy_ctas >= (1LL << 31)) return CB200_ERR_UNSUPPORTED;
   if (!a->k_cache || !a->v_cache || !a->weight_sums || !a->kv_indptr || !a->dst_indptr || !a->kept || !a->kept_sums || !a->dst_last_page_len)
     return CB200_ERR_BAD_ARG;
@@ -260,10 +336,14 @@ extern "C" int cb200_kv_evict(const cb200_kv_evict_args* a, void* stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_select_kernel, p));
+  // enough registers for the longest request that the sums or the page table can hold
+  const long long longest = static_cast<long long>(a->num_kv_indices) * a->page_size;
+  const long long guess = longest < a->max_len ? longest : a->max_len;
+  auto select = guess <= 4 * kSelThreads ? evict_select_kernel<4> : guess <= 16 * kSelThreads ? evict_select_kernel<16> : evict_select_kernel<kKeysMost>;
+  CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, select, p));
   cfg.gridDim = dim3(static_cast<unsigned>(copy_ctas), static_cast<unsigned>(a->batch), 1);
   cfg.blockDim = dim3(kCopyThreads, 1, 1);
-  CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_copy_kernel, p));
+  CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, copy_rows == 128 ? evict_copy_kernel<128> : evict_copy_kernel<32>, p));
   CB200_CUDA_TRY(cudaGetLastError());
   return CB200_OK;
 }

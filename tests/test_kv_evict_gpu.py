@@ -89,8 +89,13 @@ def test_budgets(budget, sinks, recent):
     Case(LENS, 2, 64, 16, torch.bfloat16, budget, seed=7).check(sinks, recent)
 
 
-def test_long_requests():
-    Case([9000, 4097], 2, 64, 64, torch.bfloat16, 3000, seed=8).check(4, 1000)
+@pytest.mark.parametrize("max_len", [9000, 40000, 1000])
+def test_long_requests(max_len):
+    Case([9000, 4097], 2, 64, 64, torch.bfloat16, 3000, max_len=max_len, seed=8).check(4, 1000)
+
+
+def test_requests_longer_than_a_block_holds():
+    Case([70001, 33000], 1, 64, 64, torch.bfloat16, 20000, seed=16).check(4, 1000)
 
 
 def test_more_heads_than_rows_of_a_block():
