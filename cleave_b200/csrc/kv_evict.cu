@@ -63,9 +63,9 @@ __device__ __forceinline__ Request request_of(const EvictParams& p, int b) {
 
 // Bits whose unsigned order is the order of the sums: -0 counts as 0, NaN as the largest value.
 __device__ __forceinline__ uint32_t order_key(float x) {
-  if (x != x) return 0xffffffffu;
   const uint32_t u = __float_as_uint(x + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t k = u ^ (static_cast<uint32_t>(static_cast<int>(u) >> 31) | 0x80000000u);
+  return x != x ? 0xffffffffu : k;
 }
 
 // KEYS: sums a thread holds in registers (thread t of the CTA: tokens lo + t, lo + t + 512, ...). The sums of a longer
@@ -93,29 +93,47 @@ __global__ void __launch_bounds__(kSelThreads, KEYS <= 16 ? 2 : 1) evict_select_
   auto key_of = [&](int j) { return j < hi ? order_key(sum_of(j)) : 0u; };     // no sum has the key 0
   const bool rank = middle > 0 && middle < hi - lo;
   uint32_t key[KEYS];
-  if (rank) {
+  // all loads first, none of them behind a branch: they are in flight together
+  auto load_keys = [&](int j0) {
+    float x[KEYS];
+    const int last = max(min(hi, p.max_len) - 1, 0);
 #pragma unroll
-    for (int i = 0; i < KEYS; ++i) key[i] = key_of(lo + i * kSelThreads + tid);
-  }
+    for (int i = 0; i < KEYS; ++i) x[i] = __ldg(sums + min(j0 + i * kSelThreads + tid, last));
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      const int j = j0 + i * kSelThreads + tid;
+      key[i] = j < hi ? order_key(j < p.max_len ? x[i] : 0.f) : 0u;
+    }
+  };
+  if (rank) load_keys(lo);
 
   if (h == 0 && tid == 0) p.dst_last[b] = r.keep > 0 ? (r.keep - 1) % p.page_size + 1 : 0;
-  auto put = [&](int i, int j) {
-    kept[i] = j;
-    if (i < p.max_len) kept_sums[i] = sum_of(j);
-  };
-  for (int i = tid; i < first; i += kSelThreads) put(i, i);
-  for (int i = tid; i < tail; i += kSelThreads) put(r.keep - tail + i, r.n - tail + i);
+  for (int i = tid; i < first; i += kSelThreads) kept[i] = i;
+  for (int i = tid; i < tail; i += kSelThreads) kept[r.keep - tail + i] = r.n - tail + i;
   for (int i = r.keep + tid; i < p.budget; i += kSelThreads) kept[i] = -1;
   for (int i = r.keep + tid; i < p.max_len; i += kSelThreads) kept_sums[i] = 0.f;
+  // The kept sums are copied at the end, through the indices: loads and stores of whole warps, several in flight.
+  auto carry_sums = [&]() {
+    __syncthreads();
+    const int n = min(r.keep, p.max_len);
+    for (int i0 = tid; i0 < n; i0 += 4 * kSelThreads) {
+      float x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] = i0 + u * kSelThreads < n ? sum_of(__ldcg(kept + i0 + u * kSelThreads)) : 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i0 + u * kSelThreads < n) kept_sums[i0 + u * kSelThreads] = x[u];
+    }
+  };
   if (!rank) {
-    for (int i = tid; i < middle; i += kSelThreads) put(lo + i, lo + i);
+    for (int i = tid; i < middle; i += kSelThreads) kept[lo + i] = lo + i;
+    carry_sums();
     return;
   }
 
-  auto each_key = [&](auto&& f) {  // every ranked key of this thread
+  auto each_key = [&](auto&& f) {  // every ranked key of this thread, and 0 for places behind the range
 #pragma unroll
-    for (int i = 0; i < KEYS; ++i)
-      if (lo + i * kSelThreads + tid < hi) f(key[i]);
+    for (int i = 0; i < KEYS; ++i) f(key[i]);
     for (int j = lo + KEYS * kSelThreads + tid; j < hi; j += kSelThreads) f(key_of(j));
   };
   // ---- the key of rank `middle`, by histograms over ranges of keys that shrink by kBins a round. The first range
@@ -124,7 +142,7 @@ __global__ void __launch_bounds__(kSelThreads, KEYS <= 16 ? 2 : 1) evict_select_
   // pile them up in a few bins and their counting in a few words of shared memory.
   uint32_t base = 0xffffffffu, top = 0;
   each_key([&](uint32_t k) {
-    base = min(base, k);
+    base = min(base, k - 1);  // 0 is left out
     top = max(top, k);
   });
   base = __reduce_min_sync(0xffffffffu, base);
@@ -135,14 +153,14 @@ __global__ void __launch_bounds__(kSelThreads, KEYS <= 16 ? 2 : 1) evict_select_
   }
   for (int i = tid; i < kBins; i += kSelThreads) bins[i] = 0;
   __syncthreads();
-  base = __reduce_min_sync(0xffffffffu, range[0][lane & (kWarps - 1)]);
+  base = __reduce_min_sync(0xffffffffu, range[0][lane & (kWarps - 1)]) + 1;
   top = __reduce_max_sync(0xffffffffu, range[1][lane & (kWarps - 1)]);
   int want = middle, ties = 0;  // rank inside the range; in the end: how many of the keys equal to the threshold stay
   uint32_t threshold;           // keys above it stay
   while (true) {
     const int shift = max(32 - __clz(top - base) - kBinBits, 0);
     each_key([&](uint32_t k) {
-      if (k >= base && k <= top) atomicAdd(&bins[(k - base) >> shift], 1);
+      if (k - base <= top - base) atomicAdd(&bins[(k - base) >> shift], 1);
     });
     __syncthreads();
     // a thread's four bins, largest keys first, scanned over the CTA
@@ -157,8 +175,7 @@ __global__ void __launch_bounds__(kSelThreads, KEYS <= 16 ? 2 : 1) evict_select_
     if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
     *reinterpret_cast<int4*>(&bins[kBins - 4 * (tid + 1)]) = make_int4(0, 0, 0, 0);  // for the next round
-    int above = incl - mine;
-    for (int w = 0; w < warp; ++w) above += warp_sum[w];
+    int above = incl - mine + __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
     if (above < want && want <= above + mine) {
       int bin = kBins - 1 - 4 * tid, n = c.w;
       if (above + n < want) { above += n; --bin; n = c.z; }
@@ -190,10 +207,7 @@ __global__ void __launch_bounds__(kSelThreads, KEYS <= 16 ? 2 : 1) evict_select_
   int done_strict = 0, done_tie = 0;  // before this round of slabs
   const uint32_t below = (1u << lane) - 1;
   for (int j0 = lo; j0 < hi; j0 += KEYS * kSelThreads) {
-    if (j0 > lo) {
-#pragma unroll
-      for (int i = 0; i < KEYS; ++i) key[i] = key_of(j0 + i * kSelThreads + tid);
-    }
+    if (j0 > lo) load_keys(j0);
 #pragma unroll
     for (int i = 0; i < KEYS; ++i) {
       const uint32_t bs = __ballot_sync(0xffffffffu, key[i] > threshold), bt = ties ? __ballot_sync(0xffffffffu, key[i] == threshold) : 0u;
@@ -229,12 +243,13 @@ __global__ void __launch_bounds__(kSelThreads, KEYS <= 16 ? 2 : 1) evict_select_
       const int s = done_strict + static_cast<int>(before & 0xffffu) + __popc(bs & below);
       const int t = done_tie + static_cast<int>(before >> 16) + __popc(bt & below);
       const int j = j0 + i * kSelThreads + tid;
-      if (strict || (tie && t < ties)) put(lo + s + min(t, ties), j);
+      if (strict || (tie && t < ties)) kept[lo + s + min(t, ties)] = j;
     }
     done_strict += slab_all & 0xffffu;
     done_tie += slab_all >> 16;
     __syncthreads();
   }
+  carry_sums();
 }
 
 // ROWS: (token, head) rows of K and of V per CTA
