@@ -34,6 +34,7 @@
 #include "stream_walk.cuh"
 
 #include <cstring>
+#include <type_traits>
 
 namespace cb200 {
 
@@ -439,14 +440,10 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     for (int n = 0; n < D / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
 
-    for (int ti = pc.tile0; ti < pc.tile0 + pc.count; ++ti) {
+    for (int t = pc.tile0; MODE == kPlain && t < pc.tile0 + pc.count; ++t) {
       mbar_wait(&full_bar[stage], phase, p.status, kFaultFullBarrier);
-      const int tok0 = view.tile(ti) * kTile + ws * 16;
-      // which of the warp's 16 tokens take part: some, and whether all
-      const bool some = tok0 < valid && (MODE != kWindow || tok0 + 15 >= view.lo || tok0 < p.sinks);
-      const bool all = tok0 + 15 < valid && (MODE != kWindow || tok0 >= view.lo || tok0 + 15 < p.sinks);
-      auto takes_part = [&](int tok) { return tok < valid && (MODE != kWindow || tok >= view.lo || tok < p.sinks); };
-      if (some) {
+      const int tok0 = t * kTile + ws * 16;
+      if (tok0 < valid) {
         const uint32_t kbase = stages_u32 + stage * Plan::kStageBytes;
         const uint32_t vbase = kbase + Plan::kMatBytes;
         const int mi = lane >> 3, rr = lane & 7;
@@ -471,20 +468,9 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int tok = tok0 + nb * 8 + c2 + (e & 1);
-            const float x = takes_part(tok) ? s[nb][e] * p.scale_log2 : -INFINITY;
+            const float x = tok < valid ? s[nb][e] * p.scale_log2 : -INFINITY;
             s[nb][e] = x;
             if (e < 2) mx0 = fmaxf(mx0, x); else mx1 = fmaxf(mx1, x);
-          }
-        }
-        if constexpr (MODE == kWeights) {
-          // a warp instruction writes 32-byte runs of eight rows; the scratch rows are padded to whole runs
-          float* raw = p.raw + (row_base + r0) * p.raw_pitch + tok0 + c2;
-#pragma unroll
-          for (int nb = 0; nb < 2; ++nb) {
-            if (tok0 + nb * 8 < p.raw_len) {
-              if (r0 < rows_here) *reinterpret_cast<float2*>(raw + nb * 8) = make_float2(s[nb][0], s[nb][1]);
-              if (r0 + 8 < rows_here) *reinterpret_cast<float2*>(raw + 8 * p.raw_pitch + nb * 8) = make_float2(s[nb][2], s[nb][3]);
-            }
           }
         }
         mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
@@ -496,7 +482,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         const float sc0 = fast_exp2(m_run[0] - mu0), sc1 = fast_exp2(m_run[1] - mu1);
         m_run[0] = mn0;
         m_run[1] = mn1;
-        uint32_t pf[4], pf_lo[4];
+        uint32_t pf[4];
         float ps0 = 0.f, ps1 = 0.f;
         {
           const float p00 = fast_exp2(s[0][0] - mu0), p01 = fast_exp2(s[0][1] - mu0);
@@ -509,12 +495,6 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           pf[1] = pack2<T>(p02, p03);
           pf[2] = pack2<T>(p10, p11);
           pf[3] = pack2<T>(p12, p13);
-          if constexpr (MODE != kPlain) {
-            pf_lo[0] = pack2_rest<T>(p00, p01, pf[0]);
-            pf_lo[1] = pack2_rest<T>(p02, p03, pf[1]);
-            pf_lo[2] = pack2_rest<T>(p10, p11, pf[2]);
-            pf_lo[3] = pack2_rest<T>(p12, p13, pf[3]);
-          }
         }
         l_run[0] = l_run[0] * sc0 + ps0;
         l_run[1] = l_run[1] * sc1 + ps1;
@@ -528,40 +508,176 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         // ---- O += P V
         {
           const int row = ws * 16 + (mi & 1) * 8 + rr;
-          // values of tokens that take no part become zero: 0 * V is not 0 where the row holds Inf or NaN. A
-          // register of the V fragment holds two tokens (c2, c2 + 1, or those plus 8) of one column.
-          uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-          if constexpr (MODE != kPlain) {
-            if (!all) {
-              const int tk = tok0 + c2;
-              keep0 = (takes_part(tk) ? 0xffffu : 0u) | (takes_part(tk + 1) ? 0xffff0000u : 0u);
-              keep1 = (takes_part(tk + 8) ? 0xffffu : 0u) | (takes_part(tk + 9) ? 0xffff0000u : 0u);
-            }
-          }
 #pragma unroll
           for (int dp = 0; dp < D / 16; ++dp) {
             const int d = dp * 16 + (mi >> 1) * 8;
             const uint32_t addr = vbase + (d >> 6) * (kTile * 128) + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4);
             uint32_t b0, b1, b2, b3;
             ldmatrix_x4_trans(b0, b1, b2, b3, addr);
-            if constexpr (MODE != kPlain) {
-              b0 &= keep0;
-              b1 &= keep1;
-              b2 &= keep0;
-              b3 &= keep1;
-            }
             mma_16816<T>(acc[2 * dp], pf, b0, b1);
             mma_16816<T>(acc[2 * dp + 1], pf, b2, b3);
-            if constexpr (MODE != kPlain) {
-              mma_16816<T>(acc[2 * dp], pf_lo, b0, b1);
-              mma_16816<T>(acc[2 * dp + 1], pf_lo, b2, b3);
-            }
           }
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty_bar[stage]);
       if (++stage == kStages) { stage = 0; phase ^= 1; }
+    }
+
+    // The other modes. A warp takes its 16 tokens of TWO tiles a step where all of them take part, and of one otherwise
+    // (a request's last tile, the edges of a window): with 32 tokens in hand the two chains of score MMAs overlap, and
+    // the reductions of the maximum cost half as much a token. O is rescaled only when a maximum has grown, which
+    // after the first tiles is rare; the factor would be exactly 1. (64 requests of 512..8192 tokens in 16-token pages,
+    // weights mode: 274 us a tile at a time with a rescale each, see the figures at the entry points.)
+    if constexpr (MODE != kPlain) {
+      const int mi = lane >> 3, rr = lane & 7;
+      auto takes_part = [&](int tok) { return tok < valid && (MODE != kWindow || tok >= view.lo || tok < p.sinks); };
+      auto step = [&](int ti, auto tiles, auto edge) {
+        constexpr int N = decltype(tiles)::value;
+        constexpr bool EDGE = decltype(edge)::value;  // some of the tokens may not take part
+        uint32_t kbase[N];
+        int tok0[N];
+        uint64_t* freed[N];
+        bool some = !EDGE;
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+          tok0[u] = view.tile(ti + u) * kTile + ws * 16;
+          if (EDGE) some = tok0[u] < valid && (MODE != kWindow || tok0[u] + 15 >= view.lo || tok0[u] < p.sinks);
+          kbase[u] = stages_u32 + stage * Plan::kStageBytes;
+          freed[u] = &empty_bar[stage];
+          mbar_wait(&full_bar[stage], phase, p.status, kFaultFullBarrier);
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
+        }
+        if (some) {
+          // ---- S = Q K^T
+          float s[N][2][4];
+#pragma unroll
+          for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[u][0][e] = s[u][1][e] = 0.f;
+          {
+            const int row = ws * 16 + (mi >> 1) * 8 + rr;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const int d = kk * 16 + (mi & 1) * 8;
+              const uint32_t at = (d >> 6) * (kTile * 128) + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4);
+#pragma unroll
+              for (int u = 0; u < N; ++u) {
+                uint32_t b0, b1, b2, b3;
+                ldmatrix_x4(b0, b1, b2, b3, kbase[u] + at);
+                mma_16816<T>(s[u][0], qf[kk], b0, b1);
+                mma_16816<T>(s[u][1], qf[kk], b2, b3);
+              }
+            }
+          }
+          // ---- online softmax (exp2 domain)
+          float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float x = s[u][nb][e] * p.scale_log2;
+                if (EDGE && !takes_part(tok0[u] + nb * 8 + c2 + (e & 1))) x = -INFINITY;
+                s[u][nb][e] = x;
+                if (e < 2) mx0 = fmaxf(mx0, x); else mx1 = fmaxf(mx1, x);
+              }
+          if constexpr (MODE == kWeights) {
+            // a warp instruction writes 32-byte runs of eight rows; the scratch rows are padded to whole runs
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+              float* raw = p.raw + (row_base + r0) * p.raw_pitch + tok0[u] + c2;
+#pragma unroll
+              for (int nb = 0; nb < 2; ++nb) {
+                if (tok0[u] + nb * 8 < p.raw_len) {
+                  if (r0 < rows_here) *reinterpret_cast<float2*>(raw + nb * 8) = make_float2(s[u][nb][0], s[u][nb][1]);
+                  if (r0 + 8 < rows_here) *reinterpret_cast<float2*>(raw + 8 * p.raw_pitch + nb * 8) = make_float2(s[u][nb][2], s[u][nb][3]);
+                }
+              }
+            }
+          }
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+          if (__any_sync(0xffffffffu, mx0 > m_run[0] || mx1 > m_run[1])) {
+            const float mn0 = fmaxf(m_run[0], mx0), mn1 = fmaxf(m_run[1], mx1);
+            const float sc0 = mn0 == -INFINITY ? 0.f : fast_exp2(m_run[0] - mn0), sc1 = mn1 == -INFINITY ? 0.f : fast_exp2(m_run[1] - mn1);
+            m_run[0] = mn0;
+            m_run[1] = mn1;
+            l_run[0] *= sc0;
+            l_run[1] *= sc1;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) {
+              acc[n][0] *= sc0;
+              acc[n][1] *= sc0;
+              acc[n][2] *= sc1;
+              acc[n][3] *= sc1;
+            }
+          }
+          const float mu0 = m_run[0] == -INFINITY ? 0.f : m_run[0], mu1 = m_run[1] == -INFINITY ? 0.f : m_run[1];
+#pragma unroll
+          for (int u = 0; u < N; ++u) {
+            // ---- P, as the sum of two 16-bit numbers
+            uint32_t hi[4], rest[4];
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb) {
+              const float p0 = fast_exp2(s[u][nb][0] - mu0), p1 = fast_exp2(s[u][nb][1] - mu0);
+              const float p2 = fast_exp2(s[u][nb][2] - mu1), p3 = fast_exp2(s[u][nb][3] - mu1);
+              l_run[0] += p0 + p1;
+              l_run[1] += p2 + p3;
+              hi[2 * nb] = pack2<T>(p0, p1);
+              hi[2 * nb + 1] = pack2<T>(p2, p3);
+              rest[2 * nb] = pack2_rest<T>(p0, p1, hi[2 * nb]);
+              rest[2 * nb + 1] = pack2_rest<T>(p2, p3, hi[2 * nb + 1]);
+            }
+            // ---- O += P V. Values of tokens that take no part become zero: 0 * V is not 0 where the row holds Inf or
+            // NaN. A register of the V fragment holds two tokens (c2, c2 + 1, or those plus 8) of one column.
+            uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+            if constexpr (EDGE) {
+              const int tk = tok0[u] + c2;
+              keep0 = (takes_part(tk) ? 0xffffu : 0u) | (takes_part(tk + 1) ? 0xffff0000u : 0u);
+              keep1 = (takes_part(tk + 8) ? 0xffffu : 0u) | (takes_part(tk + 9) ? 0xffff0000u : 0u);
+            }
+            const uint32_t vbase = kbase[u] + Plan::kMatBytes;
+            const int row = ws * 16 + (mi & 1) * 8 + rr;
+#pragma unroll
+            for (int dp = 0; dp < D / 16; ++dp) {
+              const int d = dp * 16 + (mi >> 1) * 8;
+              uint32_t b0, b1, b2, b3;
+              ldmatrix_x4_trans(b0, b1, b2, b3, vbase + (d >> 6) * (kTile * 128) + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4));
+              if constexpr (EDGE) {
+                b0 &= keep0;
+                b1 &= keep1;
+                b2 &= keep0;
+                b3 &= keep1;
+              }
+              mma_16816<T>(acc[2 * dp], hi, b0, b1);
+              mma_16816<T>(acc[2 * dp + 1], hi, b2, b3);
+              mma_16816<T>(acc[2 * dp], rest, b0, b1);
+              mma_16816<T>(acc[2 * dp + 1], rest, b2, b3);
+            }
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+          if (lane == 0) mbar_arrive(freed[u]);
+      };
+      auto whole = [&](int ti) {  // every token of the tile takes part (the same for the four warps)
+        const int tok = view.tile(ti) * kTile;
+        return tok + kTile <= valid && (MODE != kWindow || tok >= view.lo || tok + kTile <= p.sinks);
+      };
+      for (int ti = pc.tile0; ti < pc.tile0 + pc.count;) {
+        if (ti + 1 < pc.tile0 + pc.count && whole(ti) && whole(ti + 1)) {
+          step(ti, std::integral_constant<int, 2>{}, std::false_type{});
+          ti += 2;
+        } else {
+          step(ti, std::integral_constant<int, 1>{}, std::true_type{});
+          ti += 1;
+        }
+      }
     }
 
     // ---- merge the four warps' states through shared memory
