@@ -61,6 +61,7 @@ struct DecodeParams {
   float* partials; // gridDim.x * 2 slots
   int batch, hkv, vblk, rows, page_size, num_pages, n_idx, kv_len, paged, box_tok;
   float scale_log2;
+  int page_shift;  // log2 of page_size, or -1 where it is not a power of two
   // kWindow
   int window, sinks;
   // kWeights: scores, one row of raw_pitch floats per (request, query head); tokens beyond raw_len are not kept
@@ -71,6 +72,11 @@ struct DecodeParams {
   const float* pre_o;   // [kv head][row block][split][128][D], relative to the split's reference maximum
   const float* pre_ml;  // [kv head][row block][split][2][128]: reference maximum (log2 units), sum
   int pre_splits, pre_blocks, pre_batch;  // pre_batch: requests per row block
+};
+
+// Boxes of 16 tokens, for the tiles of which only some such groups are needed (TMA path of the modes on paged caches)
+struct GroupMaps {
+  CUtensorMap k, v;
 };
 
 template <int D, bool GATHER>
@@ -113,6 +119,17 @@ struct ItemView {
   __device__ __forceinline__ int n_tiles() const { return ceil_div(valid, kTile) - skip; }
 };
 
+// The modes read a tile in groups of 16 tokens, a consumer warp's share: whether any token of the group from `tok` on
+// takes part, and whether all 64 of the tile from `tok` on do
+template <int MODE>
+__device__ __forceinline__ bool group_lives(const DecodeParams& p, const ItemView& v, int tok) {
+  return tok < v.valid && (MODE != kWindow || tok + 15 >= v.lo || tok < p.sinks);
+}
+template <int MODE>
+__device__ __forceinline__ bool tile_whole(const DecodeParams& p, const ItemView& v, int tok) {
+  return tok + kTile <= v.valid && (MODE != kWindow || tok >= v.lo || tok + kTile <= p.sinks);
+}
+
 template <int MODE>
 __device__ __forceinline__ ItemView item_view(const DecodeParams& p, int b) {
   ItemView v{item_valid_len(p, b), 0, 0, 0};
@@ -128,7 +145,7 @@ __device__ __forceinline__ ItemView item_view(const DecodeParams& p, int b) {
 template <typename T, int D, bool GATHER, int MODE = kPlain>
 __global__ void __launch_bounds__(SmemPlan<D, GATHER>::kThreads, 1)
 decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                   const DecodeParams p) {
+                   const __grid_constant__ GroupMaps tm_group, const DecodeParams p) {
   using Plan = SmemPlan<D, GATHER>;
   constexpr int kStages = Plan::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -150,7 +167,10 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   // ---- tile prefix over requests (every CTA computes the same table)
   int tiles_per_req = 0;
   if (p.paged) {
-    pdl_wait();
+    // Behind a prefix the kernel before this one is the prefix's, which reads what this one reads, lets this one start
+    // only once its own predecessor is done, and writes nothing but the partials: they are waited for where they
+    // are merged, and CTAs that find an SM stream their requests' own tokens beside it.
+    if (MODE != kSuffix || p.pre_splits == 0) pdl_wait();
     int* scratch = reinterpret_cast<int*>(merge);  // merge buffer is free at this point
     const int per = ceil_div(p.batch, nthreads);
     const int i0 = min(tid * per, p.batch), i1 = min(i0 + per, p.batch);
@@ -230,6 +250,31 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           mbar_wait(&empty_bar[stage], phase ^ 1, p.status, kFaultEmptyBarrier);
           uint8_t* kdst = stages + stage * Plan::kStageBytes;
           uint8_t* vdst = kdst + Plan::kMatBytes;
+          if (MODE != kPlain && !tile_whole<MODE>(p, view, t * kTile)) {
+            // only the groups of 16 tokens that hold one that takes part
+            const int page_at = p.page_shift >= 0 ? (t * kTile) >> p.page_shift : t * kTile / p.page_size;
+            int page = __ldg(p.kv_indices + page_base + min(page_at, n_pages - 1));
+            page = min(max(page, 0), p.num_pages - 1);
+            const int slot = t * kTile - page_at * p.page_size;
+            uint32_t groups = 0;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) groups |= (group_lives<MODE>(p, view, t * kTile + g * 16) ? 1u : 0u) << g;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&full_bar[stage], __popc(groups) * (Plan::kStageBytes / 4));
+              for (int g = 0; g < 4; ++g) {
+                if (!(groups >> g & 1)) continue;
+#pragma unroll
+                for (int hf = 0; hf < D / 64; ++hf) {
+                  const int off = hf * (kTile * 128) + g * 16 * 128;
+                  tma_load_4d(kdst + off, &tm_group.k, &full_bar[stage], hf * 64, h, slot + g * 16, page);
+                  tma_load_4d(vdst + off, &tm_group.v, &full_bar[stage], hf * 64, h, slot + g * 16, page);
+                }
+              }
+            }
+            __syncwarp();
+            if (++stage == kStages) { stage = 0; phase ^= 1; }
+            continue;
+          }
           if (lane == 0) mbar_arrive_expect_tx(&full_bar[stage], Plan::kStageBytes);
           __syncwarp();
           if (p.paged) {
@@ -288,7 +333,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll
           for (int r = 0; r < kRounds; ++r) {
             const int tok = min(t * kTile + r * kRowsPerRound + r_in, valid - 1);
-            pg[r] = __ldg(p.kv_indices + page_base + tok / p.page_size);
+            pg[r] = __ldg(p.kv_indices + page_base + (MODE != kPlain && p.page_shift >= 0 ? tok >> p.page_shift : tok / p.page_size));
           }
         };
         int pg[kRounds];
@@ -302,11 +347,13 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           mbar_wait(&empty_bar[stage], phase ^ 1, p.status, kFaultEmptyBarrier);
           const uint32_t kdst = smem_u32(stages + stage * Plan::kStageBytes);
           const uint32_t vdst = kdst + Plan::kMatBytes;
+          const bool some = MODE != kPlain && !tile_whole<MODE>(p, view, t * kTile);
 #pragma unroll
           for (int r = 0; r < kRounds; ++r) {
             const int row = r * kRowsPerRound + r_in;
+            if (some && !group_lives<MODE>(p, view, t * kTile + (row & ~15))) continue;
             const int tok = min(t * kTile + row, valid - 1);
-            const int slot = tok - (tok / p.page_size) * p.page_size;
+            const int slot = MODE != kPlain && p.page_shift >= 0 ? tok & (p.page_size - 1) : tok - (tok / p.page_size) * p.page_size;
             const long long page = min(max(cur[r], 0), p.num_pages - 1);
             const long long off = ((page * p.page_size + slot) * p.hkv + h) * D + c * 8;
             const uint32_t dst_off = (c >> 3) * (kTile * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
@@ -352,37 +399,14 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     if (mrow >= rows_here) return;
     const size_t row = (static_cast<size_t>(b) * p.hkv + h) * p.rows + blk * kRowsMax + mrow;
     if constexpr (MODE == kSuffix) {
-      // the prefix's partials of this row, four at a time: one round trip to L2 per group
-      const size_t part0 = (static_cast<size_t>(h) * p.pre_blocks + b / p.pre_batch) * p.pre_splits;
-      const int prow = (b % p.pre_batch) * p.rows + blk * kRowsMax + mrow;
-      constexpr int kGroup = 4, kVec = kColsPerThread / 4;
-      for (int s0 = 0; s0 < p.pre_splits; s0 += kGroup) {
-        float mi_[kGroup], li_[kGroup];
-        float4 x[kGroup][kVec];
+      if (p.pre_splits > 0) {  // merge_prefix has left the prefix's sum for the item's rows in the merge buffer
+        const float Mp = merge[kRowsMax * D + mrow], Lp = merge[kRowsMax * D + kRowsMax + mrow];
+        const float Mn = fmaxf(Mf, Mp), Mu = Mn == -INFINITY ? 0.f : Mn;
+        const float fa = fast_exp2(Mf - Mu), fb = fast_exp2(Mp - Mu);
+        Lf = fa * Lf + fb * Lp;
 #pragma unroll
-        for (int g = 0; g < kGroup; ++g) {
-          const size_t part = part0 + min(s0 + g, p.pre_splits - 1);
-          mi_[g] = __ldcg(p.pre_ml + part * 256 + prow);
-          li_[g] = __ldcg(p.pre_ml + part * 256 + 128 + prow);
-#pragma unroll
-          for (int c = 0; c < kVec; ++c) x[g][c] = __ldcg(reinterpret_cast<const float4*>(p.pre_o + (part * 128 + prow) * D + mcol + 4 * c));
-        }
-#pragma unroll
-        for (int g = 0; g < kGroup; ++g) {
-          if (s0 + g >= p.pre_splits) continue;
-          const float Mn = fmaxf(Mf, mi_[g]);
-          const float Mu = Mn == -INFINITY ? 0.f : Mn;
-          const float fa = fast_exp2(Mf - Mu), fb = fast_exp2(mi_[g] - Mu);
-          Lf = fa * Lf + fb * li_[g];
-#pragma unroll
-          for (int c = 0; c < kVec; ++c) {
-            of[4 * c] = fa * of[4 * c] + fb * x[g][c].x;
-            of[4 * c + 1] = fa * of[4 * c + 1] + fb * x[g][c].y;
-            of[4 * c + 2] = fa * of[4 * c + 2] + fb * x[g][c].z;
-            of[4 * c + 3] = fa * of[4 * c + 3] + fb * x[g][c].w;
-          }
-          Mf = Mn;
-        }
+        for (int c = 0; c < kColsPerThread; ++c) of[c] = fa * of[c] + fb * merge[mrow * D + mcol + c];
+        Mf = Mn;
       }
     }
     const float inv = Lf > 0.f ? 1.f / Lf : 0.f;
@@ -398,17 +422,60 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
     if (p.lse && mcol == 0) p.lse[row] = Lf > 0.f ? Mf + fast_log2(Lf) : -INFINITY;
   };
-  if constexpr (MODE == kSuffix) {
-    // requests with nothing behind the prefix; their (request, kv head) pairs are shared out over the CTAs
-    for (int i = blockIdx.x; i < p.batch * hkvv; i += G) {
-      const int b = i / hkvv, hv = i - b * hkvv, h = hv / p.vblk, blk = hv - h * p.vblk;
-      if (P[b + 1] - P[b] != 0) continue;
-      float none[kColsPerThread];
+  // kSuffix, all consumer threads: the partials of the prefix for an item's rows, summed into the merge buffer (rows of
+  // O, then maxima and sums). A thread takes four columns of one row through all parts of the prefix, eight parts in
+  // flight, so that a group of four query heads costs one or two round trips to L2 with every thread at work.
+  auto merge_prefix = [&](int b, int h, int blk, int rows_here) {
+    if (p.pre_splits == 0) return;
+    pdl_wait();
+    named_bar_sync(1, kCThreads);  // nobody reads the buffer any more
+    const size_t part0 = (static_cast<size_t>(h) * p.pre_blocks + b / p.pre_batch) * p.pre_splits;
+    const int prow0 = (b % p.pre_batch) * p.rows + blk * kRowsMax;
+    constexpr int kGroup = 8;
+    for (int i = ctid; i < rows_here * (D / 4); i += kCThreads) {
+      const int row = i / (D / 4), col = i % (D / 4) * 4;
+      const float* ml = p.pre_ml + part0 * 256 + prow0 + row;
+      const float* o = p.pre_o + (part0 * 128 + prow0 + row) * D + col;
+      float M = -INFINITY, L = 0.f;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int s0 = 0; s0 < p.pre_splits; s0 += kGroup) {
+        float m[kGroup], l[kGroup];
+        float4 x[kGroup];
 #pragma unroll
-      for (int c = 0; c < kColsPerThread; ++c) none[c] = 0.f;
-      store_final(b, h, blk, min(kRowsMax, p.rows - blk * kRowsMax), -INFINITY, 0.f, none);
+        for (int g = 0; g < kGroup; ++g) {
+          const int s = min(s0 + g, p.pre_splits - 1);
+          m[g] = __ldcg(ml + s * 256);
+          l[g] = __ldcg(ml + s * 256 + 128);
+          x[g] = __ldcg(reinterpret_cast<const float4*>(o + static_cast<size_t>(s) * 128 * D));
+        }
+        float Mn = M;
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g) {
+          if (s0 + g >= p.pre_splits) m[g] = -INFINITY;  // a part that was loaded twice
+          Mn = fmaxf(Mn, m[g]);
+        }
+        const float Mu = Mn == -INFINITY ? 0.f : Mn, f = fast_exp2(M - Mu);
+        L *= f;
+        sum.x *= f, sum.y *= f, sum.z *= f, sum.w *= f;
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g) {
+          const float w = fast_exp2(m[g] - Mu);
+          L += w * l[g];
+          sum.x += w * x[g].x;
+          sum.y += w * x[g].y;
+          sum.z += w * x[g].z;
+          sum.w += w * x[g].w;
+        }
+        M = Mn;
+      }
+      *reinterpret_cast<float4*>(merge + row * D + col) = sum;
+      if (col == 0) {
+        merge[kRowsMax * D + row] = M;
+        merge[kRowsMax * D + kRowsMax + row] = L;
+      }
     }
-  }
+    named_bar_sync(1, kCThreads);
+  };
 
   int stage = 0, phase = 0;
   for (int u = u0; u < u1;) {
@@ -728,6 +795,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const bool starts_here = (u == pc.unit0);
     const bool whole = starts_here && pc.count == pc.n_tiles;
     if (whole) {
+      if constexpr (MODE == kSuffix) merge_prefix(pc.b, h, blk, rows_here);
       store_final(pc.b, h, blk, rows_here, M, L, o);
     } else {
       // ---- leave a partial, then let the last arriver combine
@@ -789,12 +857,27 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             }
           }
         }
+        if constexpr (MODE == kSuffix) merge_prefix(pc.b, h, blk, rows_here);
         store_final(pc.b, h, blk, rows_here, Mc, Lc, oc);
         if (ctid == 0) *counter = 0;  // ready for the next launch
       }
     }
     named_bar_sync(1, kCThreads);  // merge buffer and flag are free again
     u += pc.count;
+  }
+  if constexpr (MODE == kSuffix) {
+    // requests with nothing behind the prefix; their (request, kv head) pairs are shared out over the CTAs
+    for (int i = blockIdx.x; i < p.batch * hkvv; i += G) {
+      const int b = i / hkvv, hv = i - b * hkvv, h = hv / p.vblk, blk = hv - h * p.vblk;
+      if (P[b + 1] - P[b] != 0) continue;
+      float none[kColsPerThread];
+#pragma unroll
+      for (int c = 0; c < kColsPerThread; ++c) none[c] = 0.f;
+      const int rows_here = min(kRowsMax, p.rows - blk * kRowsMax);
+      merge_prefix(b, h, blk, rows_here);
+      store_final(b, h, blk, rows_here, -INFINITY, 0.f, none);
+    }
+    pdl_wait();  // a CTA that merged nothing: the grid is not done before the prefix's is
   }
 }
 
@@ -807,9 +890,10 @@ struct DecodeSetup {
   int grid, smem_bytes;
   size_t ws_needed, counters_off, partials_off;
   CUtensorMap tm_k, tm_v;
+  GroupMaps tm_group;
 };
 
-int plan_decode(const cb200_attn_decode_args* a, DecodeSetup* s, bool need_maps) {
+int plan_decode(const cb200_attn_decode_args* a, DecodeSetup* s, bool need_maps, bool groups = false) {
   if (!a) return CB200_ERR_BAD_ARG;
   if (a->batch <= 0 || a->num_qo_heads <= 0 || a->num_kv_heads <= 0) return CB200_ERR_BAD_ARG;
   if (a->num_qo_heads % a->num_kv_heads) return CB200_ERR_BAD_ARG;
@@ -838,6 +922,9 @@ int plan_decode(const cb200_attn_decode_args* a, DecodeSetup* s, bool need_maps)
     // small boxes per tile (measured 2.8 TB/s at 16 tokens, 4.3 at 32, 6.0 at 64) and take the row gather
     // instead (5.3 - 5.5 TB/s at any page size).
     s->gather = !(ps >= kTile && ps % kTile == 0);
+    p.page_shift = -1;
+    if ((ps & (ps - 1)) == 0)
+      for (p.page_shift = 0; (1 << p.page_shift) < ps;) ++p.page_shift;
     p.box_tok = kTile;
     tiles_ub = (static_cast<long long>(a->num_kv_indices) * ps + kTile - 1) / kTile + static_cast<long long>(a->batch) * (1 + kPieceUnits);
   } else {
@@ -909,7 +996,13 @@ int plan_decode(const cb200_attn_decode_args* a, DecodeSetup* s, bool need_maps)
     if (!encode_tensor_map(&s->tm_k, dt, 4, const_cast<void*>(a->k_cache), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !encode_tensor_map(&s->tm_v, dt, 4, const_cast<void*>(a->v_cache), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
       return CB200_ERR_CUDA;
+    memset(&s->tm_group, 0, sizeof(GroupMaps));
+    box[2] = 16u;
+    if (groups && (!encode_tensor_map(&s->tm_group.k, dt, 4, const_cast<void*>(a->k_cache), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                   !encode_tensor_map(&s->tm_group.v, dt, 4, const_cast<void*>(a->v_cache), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)))
+      return CB200_ERR_CUDA;
   } else {
+    memset(&s->tm_group, 0, sizeof(GroupMaps));
     memset(&s->tm_k, 0, sizeof(CUtensorMap));
     memset(&s->tm_v, 0, sizeof(CUtensorMap));
   }
@@ -940,7 +1033,7 @@ int launch_decode(const DecodeSetup& s, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, s.tm_k, s.tm_v, s.p));
+  CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, s.tm_k, s.tm_v, s.tm_group, s.p));
   CB200_CUDA_TRY(cudaGetLastError());
   return CB200_OK;
 }

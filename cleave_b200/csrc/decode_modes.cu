@@ -48,7 +48,7 @@ extern "C" int cb200_attn_decode_window(const cb200_attn_decode_args* a, int win
   if (!a || !a->kv_indptr || window <= 0 || sinks < 0) return CB200_ERR_BAD_ARG;
   if (a->q_rows > 1) return CB200_ERR_UNSUPPORTED;  // the window is that of one query, the request's last token
   DecodeSetup s;
-  const int rc = plan_decode(a, &s, true);
+  const int rc = plan_decode(a, &s, true, true);
   if (rc != CB200_OK) return rc;
   s.p.window = window;
   s.p.sinks = sinks;
@@ -66,7 +66,7 @@ extern "C" int cb200_attn_decode_weights(const cb200_attn_decode_args* a, float*
   if (!a || !a->kv_indptr || !a->lse || !weight_sums || max_len <= 0) return CB200_ERR_BAD_ARG;
   if (a->q_rows > 1) return CB200_ERR_UNSUPPORTED;
   DecodeSetup s;
-  const int rc = plan_decode(a, &s, true);
+  const int rc = plan_decode(a, &s, true, true);
   if (rc != CB200_OK) return rc;
   const long long pairs = static_cast<long long>(a->batch) * a->num_kv_heads;
   if (pairs > 65535) return CB200_ERR_UNSUPPORTED;

@@ -115,8 +115,8 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_holder);
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();  // not before the wait: the suffix kernel relies on what precedes this kernel being done
 
   // The 64-token boxes of tile `t` from tensor map `tm` into `dst`; boxes behind the prefix's end are not fetched.
   // Page ids come from a window of 32 that the lanes of the warp hold.
@@ -503,7 +503,7 @@ extern "C" int cb200_attn_decode_shared_prefix(const cb200_attn_decode_args* a, 
   if (!a || !a->kv_indptr || prefix_len < 0 || num_prefix_indices < 0) return CB200_ERR_BAD_ARG;
   if (a->q_rows > 1) return CB200_ERR_UNSUPPORTED;
   DecodeSetup s;
-  const int rc = plan_decode(a, &s, true);
+  const int rc = plan_decode(a, &s, true, true);
   if (rc != CB200_OK) return rc;
   if (static_cast<long long>(num_prefix_indices) * a->page_size < prefix_len) return CB200_ERR_BAD_ARG;
   if (prefix_len > (1 << 30)) return CB200_ERR_UNSUPPORTED;  // token indices are rounded up to tiles in 32 bits
