@@ -250,32 +250,16 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           mbar_wait(&empty_bar[stage], phase ^ 1, p.status, kFaultEmptyBarrier);
           uint8_t* kdst = stages + stage * Plan::kStageBytes;
           uint8_t* vdst = kdst + Plan::kMatBytes;
-          if (MODE != kPlain && !tile_whole<MODE>(p, view, t * kTile)) {
-            // only the groups of 16 tokens that hold one that takes part
-            const int page_at = p.page_shift >= 0 ? (t * kTile) >> p.page_shift : t * kTile / p.page_size;
-            int page = __ldg(p.kv_indices + page_base + min(page_at, n_pages - 1));
-            page = min(max(page, 0), p.num_pages - 1);
-            const int slot = t * kTile - page_at * p.page_size;
-            uint32_t groups = 0;
+          // an edge tile of the modes: only the groups of 16 tokens that hold one that takes part
+          uint32_t groups = 15;
+          if constexpr (MODE != kPlain) {
+            if (!tile_whole<MODE>(p, view, t * kTile)) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) groups |= (group_lives<MODE>(p, view, t * kTile + g * 16) ? 1u : 0u) << g;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&full_bar[stage], __popc(groups) * (Plan::kStageBytes / 4));
-              for (int g = 0; g < 4; ++g) {
-                if (!(groups >> g & 1)) continue;
-#pragma unroll
-                for (int hf = 0; hf < D / 64; ++hf) {
-                  const int off = hf * (kTile * 128) + g * 16 * 128;
-                  tma_load_4d(kdst + off, &tm_group.k, &full_bar[stage], hf * 64, h, slot + g * 16, page);
-                  tma_load_4d(vdst + off, &tm_group.v, &full_bar[stage], hf * 64, h, slot + g * 16, page);
-                }
-              }
+              for (int g = 0; g < 4; ++g)
+                if (!group_lives<MODE>(p, view, t * kTile + g * 16)) groups ^= 1u << g;
             }
-            __syncwarp();
-            if (++stage == kStages) { stage = 0; phase ^= 1; }
-            continue;
           }
-          if (lane == 0) mbar_arrive_expect_tx(&full_bar[stage], Plan::kStageBytes);
+          if (lane == 0) mbar_arrive_expect_tx(&full_bar[stage], MODE == kPlain ? Plan::kStageBytes : __popc(groups) * (Plan::kStageBytes / 4));
           __syncwarp();
           if (p.paged) {
             const int nbox = kTile / p.box_tok;
@@ -295,7 +279,19 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
               }
               int page = __shfl_sync(0xffffffffu, cur_idx, pord & 31);
               page = min(max(page, 0), p.num_pages - 1);
-              if (lane == 0) {
+              if (MODE != kPlain && groups != 15) {
+                if (lane == 0) {
+                  for (int g = 0; g < 4; ++g) {
+                    if (!(groups >> g & 1)) continue;
+#pragma unroll
+                    for (int hf = 0; hf < D / 64; ++hf) {
+                      const int off = hf * (kTile * 128) + g * 16 * 128;
+                      tma_load_4d(kdst + off, &tm_group.k, &full_bar[stage], hf * 64, h, slot + g * 16, page);
+                      tma_load_4d(vdst + off, &tm_group.v, &full_bar[stage], hf * 64, h, slot + g * 16, page);
+                    }
+                  }
+                }
+              } else if (lane == 0) {
 #pragma unroll
                 for (int hf = 0; hf < D / 64; ++hf) {
                   const int off = hf * (kTile * 128) + j * p.box_tok * 128;
@@ -329,39 +325,90 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         constexpr int kRowsPerRound = kPThreads / kChunks;  // rows the copying threads cover at once
         constexpr int kRounds = kTile / kRowsPerRound;
         const int c = ptid % kChunks, r_in = ptid / kChunks;
-        auto load_pages = [&](int t, int (&pg)[kRounds]) {
+        if constexpr (MODE == kPlain) {
+          auto load_pages = [&](int t, int (&pg)[kRounds]) {
 #pragma unroll
-          for (int r = 0; r < kRounds; ++r) {
-            const int tok = min(t * kTile + r * kRowsPerRound + r_in, valid - 1);
-            pg[r] = __ldg(p.kv_indices + page_base + (MODE != kPlain && p.page_shift >= 0 ? tok >> p.page_shift : tok / p.page_size));
+            for (int r = 0; r < kRounds; ++r) {
+              const int tok = min(t * kTile + r * kRowsPerRound + r_in, valid - 1);
+              pg[r] = __ldg(p.kv_indices + page_base + tok / p.page_size);
+            }
+          };
+          int pg[kRounds];
+          load_pages(pc.tile0, pg);
+          for (int t = pc.tile0; t < pc.tile0 + pc.count; ++t) {
+            int cur[kRounds];
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) cur[r] = pg[r];
+            if (t + 1 < pc.tile0 + pc.count) load_pages(t + 1, pg);
+            mbar_wait(&empty_bar[stage], phase ^ 1, p.status, kFaultEmptyBarrier);
+            const uint32_t kdst = smem_u32(stages + stage * Plan::kStageBytes);
+            const uint32_t vdst = kdst + Plan::kMatBytes;
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+              const int row = r * kRowsPerRound + r_in;
+              const int tok = min(t * kTile + row, valid - 1);
+              const int slot = tok - (tok / p.page_size) * p.page_size;
+              const long long page = min(max(cur[r], 0), p.num_pages - 1);
+              const long long off = ((page * p.page_size + slot) * p.hkv + h) * D + c * 8;
+              const uint32_t dst_off = (c >> 3) * (kTile * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(kdst + dst_off), "l"(kc + off) : "memory");
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(vdst + dst_off), "l"(vc + off) : "memory");
+            }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full_bar[stage])) : "memory");
+            if (++stage == kStages) { stage = 0; phase ^= 1; }
           }
-        };
-        int pg[kRounds];
-        load_pages(view.tile(pc.tile0), pg);
-        for (int ti = pc.tile0; ti < pc.tile0 + pc.count; ++ti) {
-          const int t = view.tile(ti);
-          int cur[kRounds];
+        } else {
+          // The copying warps are bound by the instructions they issue for an address, not by the memory: pages of a
+          // power of two of tokens are found by a shift (a division a row cost a third of the rate), a token's place in
+          // the pool is a 32-bit number (the host has checked), and only tiles at an edge look at which groups live.
+          const uint32_t row_bytes = static_cast<uint32_t>(p.hkv) * D * 2;
+          const char* kcol = reinterpret_cast<const char*>(kc + h * D + c * 8);
+          const char* vcol = reinterpret_cast<const char*>(vc + h * D + c * 8);
+          auto stream = [&](auto pow2) {
+            constexpr bool POW2 = decltype(pow2)::value;
+            auto load_pages = [&](int t, int (&pg)[kRounds]) {
 #pragma unroll
-          for (int r = 0; r < kRounds; ++r) cur[r] = pg[r];
-          if (ti + 1 < pc.tile0 + pc.count) load_pages(view.tile(ti + 1), pg);
-          mbar_wait(&empty_bar[stage], phase ^ 1, p.status, kFaultEmptyBarrier);
-          const uint32_t kdst = smem_u32(stages + stage * Plan::kStageBytes);
-          const uint32_t vdst = kdst + Plan::kMatBytes;
-          const bool some = MODE != kPlain && !tile_whole<MODE>(p, view, t * kTile);
+              for (int r = 0; r < kRounds; ++r) {
+                const int tok = min(t * kTile + r * kRowsPerRound + r_in, valid - 1);
+                pg[r] = __ldg(p.kv_indices + page_base + (POW2 ? tok >> p.page_shift : tok / p.page_size));
+              }
+            };
+            int pg[kRounds];
+            load_pages(view.tile(pc.tile0), pg);
+            for (int ti = pc.tile0; ti < pc.tile0 + pc.count; ++ti) {
+              const int t = view.tile(ti);
+              uint32_t at[kRounds];  // the rows' places in the pool
 #pragma unroll
-          for (int r = 0; r < kRounds; ++r) {
-            const int row = r * kRowsPerRound + r_in;
-            if (some && !group_lives<MODE>(p, view, t * kTile + (row & ~15))) continue;
-            const int tok = min(t * kTile + row, valid - 1);
-            const int slot = MODE != kPlain && p.page_shift >= 0 ? tok & (p.page_size - 1) : tok - (tok / p.page_size) * p.page_size;
-            const long long page = min(max(cur[r], 0), p.num_pages - 1);
-            const long long off = ((page * p.page_size + slot) * p.hkv + h) * D + c * 8;
-            const uint32_t dst_off = (c >> 3) * (kTile * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(kdst + dst_off), "l"(kc + off) : "memory");
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(vdst + dst_off), "l"(vc + off) : "memory");
-          }
-          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full_bar[stage])) : "memory");
-          if (++stage == kStages) { stage = 0; phase ^= 1; }
+              for (int r = 0; r < kRounds; ++r) {
+                const int tok = min(t * kTile + r * kRowsPerRound + r_in, valid - 1), page = min(max(pg[r], 0), p.num_pages - 1);
+                at[r] = POW2 ? (static_cast<uint32_t>(page) << p.page_shift) + (tok & (p.page_size - 1))
+                             : static_cast<uint32_t>(page) * p.page_size + tok % p.page_size;
+              }
+              if (ti + 1 < pc.tile0 + pc.count) load_pages(view.tile(ti + 1), pg);
+              mbar_wait(&empty_bar[stage], phase ^ 1, p.status, kFaultEmptyBarrier);
+              const uint32_t kdst = smem_u32(stages + stage * Plan::kStageBytes);
+              const uint32_t vdst = kdst + Plan::kMatBytes;
+              auto copy = [&](int r) {
+                const int row = r * kRowsPerRound + r_in;
+                const uint64_t off = static_cast<uint64_t>(at[r]) * row_bytes;
+                const uint32_t dst_off = (c >> 3) * (kTile * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(kdst + dst_off), "l"(kcol + off) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(vdst + dst_off), "l"(vcol + off) : "memory");
+              };
+              if (tile_whole<MODE>(p, view, t * kTile)) {
+#pragma unroll
+                for (int r = 0; r < kRounds; ++r) copy(r);
+              } else {
+#pragma unroll
+                for (int r = 0; r < kRounds; ++r)
+                  if (group_lives<MODE>(p, view, t * kTile + ((r * kRowsPerRound + r_in) & ~15))) copy(r);
+              }
+              asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full_bar[stage])) : "memory");
+              if (++stage == kStages) { stage = 0; phase ^= 1; }
+            }
+          };
+          if (p.page_shift >= 0) stream(std::true_type{});
+          else stream(std::false_type{});
         }
       }
       u += pc.count;
@@ -893,7 +940,7 @@ struct DecodeSetup {
   GroupMaps tm_group;
 };
 
-int plan_decode(const cb200_attn_decode_args* a, DecodeSetup* s, bool need_maps, bool groups = false) {
+int plan_decode(const cb200_attn_decode_args* a, DecodeSetup* s, bool need_maps, bool modes = false) {
   if (!a) return CB200_ERR_BAD_ARG;
   if (a->batch <= 0 || a->num_qo_heads <= 0 || a->num_kv_heads <= 0) return CB200_ERR_BAD_ARG;
   if (a->num_qo_heads % a->num_kv_heads) return CB200_ERR_BAD_ARG;
@@ -940,6 +987,8 @@ int plan_decode(const cb200_attn_decode_args* a, DecodeSetup* s, bool need_maps,
   const long long tiles_max = paged ? static_cast<long long>(a->batch) * ((static_cast<long long>(a->num_kv_indices) * a->page_size + kTile - 1) / kTile + 1 + kPieceUnits)
                                     : tiles_ub;
   if (tiles_max * p.hkv * p.vblk >= (1LL << 31)) return CB200_ERR_UNSUPPORTED;
+  // the modes hold a token's place in the pool in 32 bits (2^31 tokens would be 256 GB of the narrowest rows)
+  if (modes && static_cast<long long>(a->num_pages) * a->page_size >= (1LL << 31)) return CB200_ERR_UNSUPPORTED;
   const int sms = sm_count();
   if (sms <= 0) return CB200_ERR_CUDA;
   int grid = sms;
@@ -998,7 +1047,7 @@ int plan_decode(const cb200_attn_decode_args* a, DecodeSetup* s, bool need_maps,
       return CB200_ERR_CUDA;
     memset(&s->tm_group, 0, sizeof(GroupMaps));
     box[2] = 16u;
-    if (groups && (!encode_tensor_map(&s->tm_group.k, dt, 4, const_cast<void*>(a->k_cache), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+    if (modes && (!encode_tensor_map(&s->tm_group.k, dt, 4, const_cast<void*>(a->k_cache), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
                    !encode_tensor_map(&s->tm_group.v, dt, 4, const_cast<void*>(a->v_cache), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)))
       return CB200_ERR_CUDA;
   } else {
