@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(_HERE, "libcleave_b200.so")
 F16, BF16 = 0, 1
 OK = 0
 ERR_UNSUPPORTED = 2
+ERR_WORKSPACE = 4
 ERR_DEVICE_TIMEOUT = 6
 
 

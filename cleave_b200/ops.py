@@ -143,45 +143,89 @@ def gqa_paged_decode(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_le
     return out, lse
 
 
-def _one_device(**tensors) -> None:
-    """Refuses tensors that are not all on the device of the first one."""
-    first, where = None, None
+def _raw_stream(index: int) -> int:
+    """The current stream's handle on device ``index`` (:func:`_stream` builds a Stream object for it, which takes a
+    microsecond)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _check_all(device, **tensors) -> None:
+    """Refuses tensors that are not contiguous or not on ``device``."""
     for name, t in tensors.items():
-        if t is None:
-            continue
-        if first is None:
-            first, where = name, t.device
-        elif t.device != where:
-            raise ValueError(f"{name} must be on {first}'s device ({where}, not {t.device})")
+        if t is not None and (t.device != device or not t.is_contiguous()):
+            _cuda(t, name)
+            raise ValueError(f"{name} must be on {device}, not on {t.device}")
 
 
-def _launch_workspace(kind: str, nbytes: int, device) -> torch.Tensor:
-    """:func:`workspace`, except while the stream is being captured: two graphs that were captured on one stream may be
-    replayed beside each other, so each call in a graph gets a workspace of its own from the graph's pool, which the
-    graph zero-fills in front of the launch."""
-    if not torch.cuda.is_current_stream_capturing():
-        return workspace(kind, nbytes, device)
+def _private_workspace(nbytes: int, device) -> torch.Tensor:
+    """A workspace for one call in a graph under capture. Two graphs that were captured on one stream may be replayed beside
+    each other, so they must not share the stream's workspace: the call gets one from the graph's pool, which the graph
+    zero-fills in front of the launch."""
     ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
     _lib.check(_lib.lib().cb200_workspace_reset(ws.data_ptr(), ws.numel(), _stream()))
     return ws
 
 
+def _launch(kind, a, nbytes_of, device, stream, launch) -> None:
+    """``launch()`` with a workspace in the argument struct ``a``: the one that is cached for (kind, device, stream), after
+    asking ``nbytes_of`` for the size where there is none or it is too small; under capture a private one."""
+    if torch.cuda.is_current_stream_capturing():
+        need = nbytes_of(C.byref(a))
+        ws = _private_workspace(need, device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        _lib.check(launch())
+        return
+    ws = _workspaces.get((kind, device.index, stream))
+    if ws is not None:
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        status = launch()
+        if status != _lib.ERR_WORKSPACE:
+            return _lib.check(status)
+    need = nbytes_of(C.byref(a))  # 0 where the arguments are refused: the launch says why
+    ws = workspace(kind, need, device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _lib.check(launch())
+
+
 def _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, out, lse, max_ctas):
-    """Outputs, checked arguments and workspace of the paged decode variants, on the current device: (out, lse, args,
-    workspace); the caller keeps the workspace alive until it has launched."""
+    """The checked arguments of the paged decode variants, and their outputs: (out, lse, args). The same refusals as
+    :func:`_paged_decode_args`, and every tensor has to be on q's device; written for calls whose kernel takes a few
+    microseconds."""
+    device, dtype = q.device, q.dtype
+    _check_all(device, q=q, k_cache=k_cache, v_cache=v_cache, kv_indptr=kv_indptr, kv_indices=kv_indices,
+               kv_last_page_len=kv_last_page_len, out=out, lse=lse)
+    if q.dim() != 3 or k_cache.dim() != 4:
+        raise ValueError("q must be (batch, HQ, D) and the caches (num_pages, page_size, HKV, D)")
+    batch, hq, d = q.shape
+    num_pages, page_size, hkv, d2 = shape = k_cache.shape
+    if d2 != d or v_cache.shape != shape:
+        raise ValueError("k_cache / v_cache must be (num_pages, page_size, HKV, D) with q's D")
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise TypeError("q and the caches must share one storage dtype")
+    if kv_indptr.dtype != torch.int32 or kv_indices.dtype != torch.int32:
+        raise TypeError("kv_indptr / kv_indices must be int32")
+    if kv_indptr.numel() != batch + 1:
+        raise ValueError("kv_indptr must have batch + 1 entries")
+    last = None
+    if kv_last_page_len is not None:
+        if kv_last_page_len.dtype != torch.int32 or kv_last_page_len.numel() != batch:
+            raise TypeError("kv_last_page_len must hold batch int32 values")
+        last = kv_last_page_len.data_ptr()
+    elif page_size != 1:
+        raise TypeError("missing input 'kv_last_page_len'")
+    code = _dtype_code(q)
     if out is None:
         out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != dtype:
+        raise ValueError("out must have q's shape, dtype and device")
     if lse is None:
-        lse = torch.empty(tuple(q.shape[:2]), dtype=torch.float32, device=q.device)
-    _one_device(q=q, k_cache=k_cache, v_cache=v_cache, kv_indptr=kv_indptr, kv_indices=kv_indices,
-                kv_last_page_len=kv_last_page_len)
-    a = _paged_decode_args(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, out, lse, max_ctas)
-    need = _lib.lib().cb200_attn_decode_workspace_bytes(C.byref(a))
-    if need == 0:
-        _lib.check(_lib.lib().cb200_attn_decode(C.byref(a), _stream()))  # raises the real status
-    ws = _launch_workspace("attn_decode", need, q.device)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    return out, lse, a, ws
+        lse = torch.empty((batch, hq), dtype=torch.float32, device=device)
+    elif tuple(lse.shape) != (batch, hq) or lse.dtype != torch.float32:
+        raise ValueError("lse must be (batch, HQ) float32 on q's device")
+    a = _lib.AttnDecodeArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), last,
+                            out.data_ptr(), lse.data_ptr(), None, 0, batch, hq, hkv, d, page_size, num_pages, kv_indices.numel(),
+                            0, 1, code, max_ctas, sm_scale)
+    return out, lse, a
 
 
 def _window_args(window, sinks):
@@ -203,9 +247,10 @@ def gqa_paged_decode_window(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_
         with torch.cuda.device(q.device):
             return gqa_paged_decode_window(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, window,
                                            sinks, out=out, lse=lse, max_ctas=max_ctas)
-    out, lse, a, ws = _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, out, lse,
-                                          max_ctas)
-    _lib.check(_lib.lib().cb200_attn_decode_window(C.byref(a), window, sinks, _stream()))
+    out, lse, a = _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, out, lse, max_ctas)
+    L, stream = _lib.lib(), _raw_stream(q.device.index)
+    _launch("attn_decode", a, L.cb200_attn_decode_workspace_bytes, q.device, stream,
+            lambda: L.cb200_attn_decode_window(C.byref(a), window, sinks, stream))
     return out, lse
 
 
@@ -222,18 +267,18 @@ def gqa_paged_decode_weights(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last
         with torch.cuda.device(q.device):
             return gqa_paged_decode_weights(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale,
                                             weight_sums, out=out, lse=lse, max_ctas=max_ctas)
-    _one_device(q=q, weight_sums=weight_sums)
-    out, lse, a, ws = _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, out, lse,
-                                          max_ctas)
-    if _cuda(weight_sums, "weight_sums").dtype != torch.float32:
+    _check_all(q.device, weight_sums=weight_sums)
+    out, lse, a = _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, out, lse, max_ctas)
+    if weight_sums.dtype != torch.float32:
         raise TypeError("weight_sums must be float32")
     if weight_sums.dim() != 3 or tuple(weight_sums.shape[:2]) != (q.shape[0], k_cache.shape[2]):
         raise ValueError("weight_sums must be (batch, HKV, max_len)")
     max_len = weight_sums.shape[2]
-    scratch = torch.empty(_lib.lib().cb200_attn_decode_weights_scratch_bytes(C.byref(a), max_len), dtype=torch.uint8,
-                          device=q.device)
-    _lib.check(_lib.lib().cb200_attn_decode_weights(C.byref(a), weight_sums.data_ptr(), max_len, scratch.data_ptr(),
-                                                    scratch.numel(), _stream()))
+    L, stream = _lib.lib(), _raw_stream(q.device.index)
+    need = L.cb200_attn_decode_weights_scratch_bytes(C.byref(a), max_len)
+    scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _launch("attn_decode", a, L.cb200_attn_decode_workspace_bytes, q.device, stream,
+            lambda: L.cb200_attn_decode_weights(C.byref(a), weight_sums.data_ptr(), max_len, scratch.data_ptr(), need, stream))
     return out, lse
 
 
@@ -249,18 +294,18 @@ def gqa_paged_decode_shared_prefix(q, k_cache, v_cache, prefix_indices, prefix_l
             return gqa_paged_decode_shared_prefix(q, k_cache, v_cache, prefix_indices, prefix_len, kv_indptr, kv_indices,
                                                   kv_last_page_len, sm_scale, out=out, lse=lse, max_ctas=max_ctas)
     prefix_len = int(prefix_len)
-    _one_device(q=q, prefix_indices=_cuda(prefix_indices, "prefix_indices"))
-    out, lse, a, ws = _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, out, lse,
-                                          max_ctas)
+    _check_all(q.device, prefix_indices=prefix_indices)
+    out, lse, a = _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, out, lse, max_ctas)
     if prefix_indices.dtype != torch.int32:
         raise TypeError("prefix_indices must be int32")
     if prefix_len < 0 or prefix_len > prefix_indices.numel() * k_cache.shape[1]:
         raise ValueError(f"prefix_len must be between 0 and the {prefix_indices.numel()} pages of prefix_indices, got {prefix_len}")
-    L = _lib.lib()
+    L, stream = _lib.lib(), _raw_stream(q.device.index)
     need = L.cb200_attn_decode_shared_prefix_scratch_bytes(C.byref(a), prefix_len)
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _lib.check(L.cb200_attn_decode_shared_prefix(C.byref(a), prefix_indices.data_ptr(), prefix_indices.numel(), prefix_len,
-                                                 scratch.data_ptr(), need, _stream()))
+    _launch("attn_decode", a, L.cb200_attn_decode_workspace_bytes, q.device, stream,
+            lambda: L.cb200_attn_decode_shared_prefix(C.byref(a), prefix_indices.data_ptr(), prefix_indices.numel(), prefix_len,
+                                                      scratch.data_ptr(), need, stream))
     return out, lse
 
 
@@ -280,9 +325,9 @@ def kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last
         with torch.cuda.device(k_cache.device):
             return kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last_page_len, dst_indptr, dst_indices,
                                   budget=budget, sinks=sinks, recent=recent)
-    _cuda(v_cache, "v_cache"), _cuda(weight_sums, "weight_sums")
-    _one_device(k_cache=k_cache, v_cache=v_cache, weight_sums=weight_sums, kv_indptr=kv_indptr, kv_indices=kv_indices,
-                kv_last_page_len=kv_last_page_len, dst_indptr=dst_indptr, dst_indices=dst_indices)
+    device = k_cache.device
+    _check_all(device, v_cache=v_cache, weight_sums=weight_sums, kv_indptr=kv_indptr, kv_indices=kv_indices,
+               kv_last_page_len=kv_last_page_len, dst_indptr=dst_indptr, dst_indices=dst_indices)
     budget, sinks, recent = int(budget), int(sinks), int(recent)
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"budget must be at least 1 and at least sinks + recent, got {budget}, {sinks} and {recent}")
@@ -295,31 +340,25 @@ def kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last
     if weight_sums.dim() != 3 or weight_sums.shape[1] != hkv:
         raise ValueError("weight_sums must be (batch, HKV, max_len)")
     batch, _, max_len = weight_sums.shape
-    tables = {"kv_indptr": kv_indptr, "kv_indices": kv_indices, "dst_indptr": dst_indptr, "dst_indices": dst_indices}
-    if page_size != 1 and kv_last_page_len is None:
+    if kv_last_page_len is None and page_size != 1:
         raise TypeError("missing input 'kv_last_page_len'")
-    if kv_last_page_len is not None:
-        tables["kv_last_page_len"] = kv_last_page_len
-    for name, t in tables.items():
-        if _cuda(t, name).dtype != torch.int32:
-            raise TypeError(f"{name} must be int32")
+    i32 = torch.int32
+    if kv_indptr.dtype != i32 or kv_indices.dtype != i32 or dst_indptr.dtype != i32 or dst_indices.dtype != i32:
+        raise TypeError("kv_indptr, kv_indices, dst_indptr and dst_indices must be int32")
+    if kv_last_page_len is not None and kv_last_page_len.dtype != i32:
+        raise TypeError("kv_last_page_len must be int32")
     if kv_indptr.numel() != batch + 1 or dst_indptr.numel() != batch + 1:
         raise ValueError("kv_indptr and dst_indptr must have batch + 1 entries")
     if kv_last_page_len is not None and kv_last_page_len.numel() != batch:
         raise ValueError("kv_last_page_len must hold batch values")
-    kept = torch.empty((batch, hkv, budget), dtype=torch.int32, device=k_cache.device)
+    kept = torch.empty((batch, hkv, budget), dtype=i32, device=device)
     sums = torch.empty_like(weight_sums)
-    last = torch.empty(batch, dtype=torch.int32, device=k_cache.device)
-    a = _lib.KvEvictArgs()
-    a.k_cache, a.v_cache, a.weight_sums = k_cache.data_ptr(), v_cache.data_ptr(), weight_sums.data_ptr()
-    a.kv_indptr, a.kv_indices = kv_indptr.data_ptr(), kv_indices.data_ptr()
-    a.kv_last_page_len = None if kv_last_page_len is None else kv_last_page_len.data_ptr()
-    a.dst_indptr, a.dst_indices = dst_indptr.data_ptr(), dst_indices.data_ptr()
-    a.kept, a.kept_sums, a.dst_last_page_len = kept.data_ptr(), sums.data_ptr(), last.data_ptr()
-    a.batch, a.num_kv_heads, a.head_dim, a.page_size, a.num_pages = batch, hkv, d, page_size, num_pages
-    a.num_kv_indices, a.num_dst_indices, a.max_len = kv_indices.numel(), dst_indices.numel(), max_len
-    a.budget, a.sinks, a.recent = budget, sinks, recent
-    _lib.check(_lib.lib().cb200_kv_evict(C.byref(a), _stream()))
+    last = torch.empty(batch, dtype=i32, device=device)
+    a = _lib.KvEvictArgs(k_cache.data_ptr(), v_cache.data_ptr(), weight_sums.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(),
+                         None if kv_last_page_len is None else kv_last_page_len.data_ptr(), dst_indptr.data_ptr(),
+                         dst_indices.data_ptr(), kept.data_ptr(), sums.data_ptr(), last.data_ptr(), batch, hkv, d, page_size,
+                         num_pages, kv_indices.numel(), dst_indices.numel(), max_len, budget, sinks, recent)
+    _lib.check(_lib.lib().cb200_kv_evict(C.byref(a), _raw_stream(device.index)))
     return kept, sums, last
 
 
@@ -516,32 +555,25 @@ def gqa_paged_prefill(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_
 
 
 def _prefill_window(q, k, v, qo_indptr, kv_indptr, kv_indices, sm_scale, window, sinks, out, lse):
+    device = q.device
     total_q, hq, d = q.shape
-    total_kv, hkv, _ = k.shape
-    a = _lib.AttnPrefillRaggedArgs()
     fill = (1 if out is None else 0) | (2 if lse is None else 0)
     if out is None:
         out = torch.empty_like(q)
-    if lse is None:
-        lse = torch.empty((total_q, hq), dtype=torch.float32, device=q.device)
-    if _cuda(out, "out").shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+    elif out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("out must have q's shape, dtype and device")
-    if tuple(_cuda(lse, "lse").shape) != (total_q, hq) or lse.dtype != torch.float32 or lse.device != q.device:
+    if lse is None:
+        lse = torch.empty((total_q, hq), dtype=torch.float32, device=device)
+    elif tuple(lse.shape) != (total_q, hq) or lse.dtype != torch.float32:
         raise ValueError("lse must be (total_q, HQ) float32 on q's device")
-    a.q, a.k, a.v, a.out, a.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr()
-    a.qo_indptr, a.kv_indptr = qo_indptr.data_ptr(), kv_indptr.data_ptr()
-    if kv_indices is not None:
-        a.kv_indices, a.num_kv_indices = kv_indices.data_ptr(), kv_indices.numel()
-    a.batch, a.total_q, a.total_kv = qo_indptr.numel() - 1, total_q, total_kv
-    a.num_qo_heads, a.num_kv_heads, a.head_dim = hq, hkv, d
-    a.dtype, a.causal, a.sm_scale = _dtype_code(q), 1, float(sm_scale)
-    L = _lib.lib()
-    need = L.cb200_attn_prefill_ragged_workspace_bytes(C.byref(a))
-    if need == 0:
-        _lib.check(L.cb200_attn_prefill_ragged_window(C.byref(a), window, sinks, fill, _stream()))  # raises the real status
-    ws = _launch_workspace("attn_prefill", need, q.device)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    _lib.check(L.cb200_attn_prefill_ragged_window(C.byref(a), window, sinks, fill, _stream()))
+    paged = kv_indices is not None
+    a = _lib.AttnPrefillRaggedArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), qo_indptr.data_ptr(), kv_indptr.data_ptr(),
+                                   kv_indices.data_ptr() if paged else None, out.data_ptr(), lse.data_ptr(), None, 0,
+                                   qo_indptr.numel() - 1, total_q, k.shape[0], hq, k.shape[-2], d, _dtype_code(q), 1, sm_scale,
+                                   kv_indices.numel() if paged else 0)
+    L, stream = _lib.lib(), _raw_stream(device.index)
+    _launch("attn_prefill", a, L.cb200_attn_prefill_ragged_workspace_bytes, device, stream,
+            lambda: L.cb200_attn_prefill_ragged_window(C.byref(a), window, sinks, fill, stream))
     return out, lse
 
 
@@ -554,16 +586,15 @@ def gqa_ragged_prefill_window(q, k, v, qo_indptr, kv_indptr, sm_scale, window, s
     if _cuda(q, "q").device.index != torch.cuda.current_device():
         with torch.cuda.device(q.device):
             return gqa_ragged_prefill_window(q, k, v, qo_indptr, kv_indptr, sm_scale, window, sinks, out=out, lse=lse)
-    _cuda(k, "k"), _cuda(v, "v")
+    _check_all(q.device, k=k, v=v, qo_indptr=qo_indptr, kv_indptr=kv_indptr, out=out, lse=lse)
     if q.dim() != 3 or k.dim() != 3 or k.shape[2] != q.shape[2] or v.shape != k.shape or k.shape[1] == 0 or q.shape[1] % k.shape[1]:
         raise ValueError("shapes: q (total_q,HQ,D), k/v (total_kv,HKV,D), HQ a multiple of HKV")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError("q, k and v must share one storage dtype")
-    if _cuda(qo_indptr, "qo_indptr").dtype != torch.int32 or _cuda(kv_indptr, "kv_indptr").dtype != torch.int32:
+    if qo_indptr.dtype != torch.int32 or kv_indptr.dtype != torch.int32:
         raise TypeError("qo_indptr / kv_indptr must be int32")
     if qo_indptr.numel() < 2 or qo_indptr.numel() != kv_indptr.numel():
         raise ValueError("qo_indptr and kv_indptr must both hold batch + 1 entries")
-    _one_device(q=q, k=k, v=v, qo_indptr=qo_indptr, kv_indptr=kv_indptr)
     return _prefill_window(q, k, v, qo_indptr, kv_indptr, None, sm_scale, window, sinks, out, lse)
 
 
@@ -577,22 +608,21 @@ def gqa_paged_prefill_window(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indic
         with torch.cuda.device(q.device):
             return gqa_paged_prefill_window(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_scale, window, sinks, out=out,
                                             lse=lse)
-    _cuda(k_cache, "k_cache"), _cuda(v_cache, "v_cache")
+    _check_all(q.device, k_cache=k_cache, v_cache=v_cache, qo_indptr=qo_indptr, kv_indptr=kv_indptr, kv_indices=kv_indices, out=out,
+               lse=lse)
     if k_cache.dim() != 4 or k_cache.shape[1] != 1 or v_cache.shape != k_cache.shape:
         raise ValueError("caches: (num_pages, 1, HKV, D), one token per page")
     if q.dim() != 3 or k_cache.shape[3] != q.shape[2] or k_cache.shape[2] == 0 or q.shape[1] % k_cache.shape[2]:
         raise ValueError("shapes: q (total_q,HQ,D), caches (num_pages,1,HKV,D), HQ a multiple of HKV")
     if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
         raise TypeError("q and the caches must share one storage dtype")
-    for name, t in (("qo_indptr", qo_indptr), ("kv_indptr", kv_indptr), ("kv_indices", kv_indices)):
-        if _cuda(t, name).dtype != torch.int32:
-            raise TypeError(f"{name} must be int32")
+    if qo_indptr.dtype != torch.int32 or kv_indptr.dtype != torch.int32 or kv_indices.dtype != torch.int32:
+        raise TypeError("qo_indptr / kv_indptr / kv_indices must be int32")
     if kv_indices.numel() == 0:
         raise ValueError("kv_indices must hold at least one page")
     if qo_indptr.numel() < 2 or qo_indptr.numel() != kv_indptr.numel():
         raise ValueError("qo_indptr and kv_indptr must both hold batch + 1 entries")
-    _one_device(q=q, k_cache=k_cache, v_cache=v_cache, qo_indptr=qo_indptr, kv_indptr=kv_indptr, kv_indices=kv_indices)
-    return _prefill_window(q, k_cache[:, 0], v_cache[:, 0], qo_indptr, kv_indptr, kv_indices, sm_scale, window, sinks, out, lse)
+    return _prefill_window(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_scale, window, sinks, out, lse)
 
 
 def gqa_paged_decode_static_scratch(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale,
