@@ -79,7 +79,7 @@ struct GroupMaps {
   CUtensorMap k, v;
 };
 
-template <int D, bool GATHER>
+template <int D, bool GATHER, int MODE>
 struct SmemPlan {
   // Both paths use the same tile layout: per 64-column half, 64 rows of 128 bytes with the
   // 128-byte swizzle (what TMA writes; the gather path reproduces it with 16-byte cp.async).
@@ -90,7 +90,11 @@ struct SmemPlan {
   // over random 1 KB rows moved 4.0 TB/s with four warps per SM whatever their depth, 6.0 with eight)
   static constexpr int kProducerWarps = GATHER ? 8 : 1;
   static constexpr int kThreads = (kConsumerWarps + kProducerWarps) * 32;
-  static constexpr int kMergeFloats = kRowsMax * D + 2 * kRowsMax;
+  // A warp's state in the merge buffer. In the modes the rows are eight floats apart in the banks, so that the fragments'
+  // rows meet no bank twice when they are written (the plain kernel's rows of D floats leave room for more requests).
+  static constexpr int kMergePitch = MODE == kPlain ? D : D + 8;
+  static constexpr int kMergeFloats = kRowsMax * kMergePitch + 2 * kRowsMax;
+  static constexpr int kSlotFloats = kRowsMax * D + 2 * kRowsMax;  // a partial in the workspace
   static constexpr int kMergeBytes = kConsumerWarps * kMergeFloats * 4;
   static constexpr int kFixedBytes = kStages * kStageBytes + kMergeBytes + 256;  // + barriers/flags
 };
@@ -111,42 +115,58 @@ __device__ __forceinline__ int item_valid_len(const DecodeParams& p, int b) {
   return max(min(v, n_pages * p.page_size), 0);
 }
 
-// The tiles of a request that are in the stream: tile t of the item is tile t of the cache while t < n_sink, and
-// tile t + skip behind that. Tokens from `lo` on are inside the window.
+// The tiles of a request with n tokens that are in the stream. Whole boxes of the cache (TMA): tile t of the item is tile t
+// of the cache while t < n_sink, and tile t + skip behind that; tokens from `lo` on are inside the window, and the tiles
+// at the edges hold others too. Gathered rows: the stream holds the tokens that take part and no others; its token v is
+// the cache's v while v < head, and v + jump behind that.
 struct ItemView {
-  int valid, lo, n_sink, skip;
+  int valid;               // tokens up to which the stream's count runs
+  int lo, n_sink, skip;    // whole boxes
+  int head, jump;          // gathered rows
   __device__ __forceinline__ int tile(int t) const { return t < n_sink ? t : t + skip; }
+  __device__ __forceinline__ int token(int v) const { return v < head ? v : v + jump; }
   __device__ __forceinline__ int n_tiles() const { return ceil_div(valid, kTile) - skip; }
 };
 
-// The modes read a tile in groups of 16 tokens, a consumer warp's share: whether any token of the group from `tok` on
-// takes part, and whether all 64 of the tile from `tok` on do
-template <int MODE>
-__device__ __forceinline__ bool group_lives(const DecodeParams& p, const ItemView& v, int tok) {
-  return tok < v.valid && (MODE != kWindow || tok + 15 >= v.lo || tok < p.sinks);
-}
-template <int MODE>
-__device__ __forceinline__ bool tile_whole(const DecodeParams& p, const ItemView& v, int tok) {
-  return tok + kTile <= v.valid && (MODE != kWindow || tok >= v.lo || tok + kTile <= p.sinks);
-}
-
-template <int MODE>
-__device__ __forceinline__ ItemView item_view(const DecodeParams& p, int b) {
-  ItemView v{item_valid_len(p, b), 0, 0, 0};
+template <int MODE, bool GATHER>
+__device__ __forceinline__ ItemView item_view(const DecodeParams& p, int n) {
+  ItemView v{n, 0, 0, 0, 0, 0};
   if constexpr (MODE == kWindow) {
-    v.lo = max(v.valid - p.window, 0);
-    const int first = v.lo / kTile;
-    v.n_sink = min(ceil_div(min(p.sinks, v.lo), kTile), first);
-    v.skip = first - v.n_sink;
+    const int lo = max(n - p.window, 0), sinks = min(p.sinks, lo);
+    if constexpr (GATHER) {
+      v.head = sinks;
+      v.jump = lo - sinks;
+      v.valid = n - v.jump;
+    } else {
+      const int first = lo / kTile;
+      v.lo = lo;
+      v.n_sink = min(ceil_div(sinks, kTile), first);
+      v.skip = first - v.n_sink;
+    }
   }
   return v;
 }
 
+// The modes read a tile in groups of 16 tokens, a consumer warp's share: whether token `tok` takes part, whether any of the
+// group from `tok` on does, and whether all 64 of the tile from `tok` on do
+template <int MODE, bool GATHER>
+__device__ __forceinline__ bool token_lives(const DecodeParams& p, const ItemView& v, int tok) {
+  return tok < v.valid && (MODE != kWindow || GATHER || tok >= v.lo || tok < p.sinks);
+}
+template <int MODE, bool GATHER>
+__device__ __forceinline__ bool group_lives(const DecodeParams& p, const ItemView& v, int tok) {
+  return tok < v.valid && (MODE != kWindow || GATHER || tok + 15 >= v.lo || tok < p.sinks);
+}
+template <int MODE, bool GATHER>
+__device__ __forceinline__ bool tile_whole(const DecodeParams& p, const ItemView& v, int tok) {
+  return tok + kTile <= v.valid && (MODE != kWindow || GATHER || tok >= v.lo || tok + kTile <= p.sinks);
+}
+
 template <typename T, int D, bool GATHER, int MODE = kPlain>
-__global__ void __launch_bounds__(SmemPlan<D, GATHER>::kThreads, 1)
+__global__ void __launch_bounds__(SmemPlan<D, GATHER, MODE>::kThreads, 1)
 decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                    const __grid_constant__ GroupMaps tm_group, const DecodeParams p) {
-  using Plan = SmemPlan<D, GATHER>;
+  using Plan = SmemPlan<D, GATHER, MODE>;
   constexpr int kStages = Plan::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -156,6 +176,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   uint64_t* empty_bar = full_bar + kStages;
   int* flags = reinterpret_cast<int*>(empty_bar + kStages);  // [0] last-arriver flag, [1..] scan scratch
   int* P = reinterpret_cast<int*>(smem + Plan::kFixedBytes);
+  int* V = P + p.batch + 1;  // modes: tokens per request, so that a piece is found without a trip to memory
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nthreads = blockDim.x;
@@ -175,7 +196,11 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const int per = ceil_div(p.batch, nthreads);
     const int i0 = min(tid * per, p.batch), i1 = min(i0 + per, p.batch);
     int sum = 0;
-    for (int i = i0; i < i1; ++i) sum += Walker::units(item_view<MODE>(p, i).n_tiles(), kPieceUnits);
+    for (int i = i0; i < i1; ++i) {
+      const int n = item_valid_len(p, i);
+      if (MODE != kPlain) V[i] = n;
+      sum += Walker::units(item_view<MODE, GATHER>(p, n).n_tiles(), kPieceUnits);
+    }
     scratch[tid] = sum;
     __syncthreads();
     if (tid < 32) {
@@ -186,7 +211,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     int run = scratch[tid];
     for (int i = i0; i < i1; ++i) {
       P[i] = run;
-      run += Walker::units(item_view<MODE>(p, i).n_tiles(), kPieceUnits);
+      run += Walker::units(item_view<MODE, GATHER>(p, MODE != kPlain ? V[i] : item_valid_len(p, i)).n_tiles(), kPieceUnits);
     }
   } else {
     tiles_per_req = ceil_div(p.kv_len, kTile);
@@ -239,7 +264,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       const Piece pc = walker.at(u, u1);
       if (pc.count == 0) break;  // the share ends in front of the next item's tiles
       const int h = pc.hv / p.vblk;
-      const ItemView view = item_view<MODE>(p, pc.b);
+      const ItemView view = item_view<MODE, GATHER>(p, MODE != kPlain ? V[pc.b] : item_valid_len(p, pc.b));
       const int valid = view.valid;
       const int page_base = p.paged ? p.kv_indptr[pc.b] : 0;
       const int n_pages = p.paged ? ceil_div(valid, p.page_size) : 0;
@@ -253,10 +278,10 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           // an edge tile of the modes: only the groups of 16 tokens that hold one that takes part
           uint32_t groups = 15;
           if constexpr (MODE != kPlain) {
-            if (!tile_whole<MODE>(p, view, t * kTile)) {
+            if (!tile_whole<MODE, GATHER>(p, view, t * kTile)) {
 #pragma unroll
               for (int g = 0; g < 4; ++g)
-                if (!group_lives<MODE>(p, view, t * kTile + g * 16)) groups ^= 1u << g;
+                if (!group_lives<MODE, GATHER>(p, view, t * kTile + g * 16)) groups ^= 1u << g;
             }
           }
           if (lane == 0) mbar_arrive_expect_tx(&full_bar[stage], MODE == kPlain ? Plan::kStageBytes : __popc(groups) * (Plan::kStageBytes / 4));
@@ -369,7 +394,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             auto load_pages = [&](int t, int (&pg)[kRounds]) {
 #pragma unroll
               for (int r = 0; r < kRounds; ++r) {
-                const int tok = min(t * kTile + r * kRowsPerRound + r_in, valid - 1);
+                const int tok = view.token(min(t * kTile + r * kRowsPerRound + r_in, valid - 1));
                 pg[r] = __ldg(p.kv_indices + page_base + (POW2 ? tok >> p.page_shift : tok / p.page_size));
               }
             };
@@ -380,7 +405,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
               uint32_t at[kRounds];  // the rows' places in the pool
 #pragma unroll
               for (int r = 0; r < kRounds; ++r) {
-                const int tok = min(t * kTile + r * kRowsPerRound + r_in, valid - 1), page = min(max(pg[r], 0), p.num_pages - 1);
+                const int tok = view.token(min(t * kTile + r * kRowsPerRound + r_in, valid - 1)), page = min(max(pg[r], 0), p.num_pages - 1);
                 at[r] = POW2 ? (static_cast<uint32_t>(page) << p.page_shift) + (tok & (p.page_size - 1))
                              : static_cast<uint32_t>(page) * p.page_size + tok % p.page_size;
               }
@@ -395,13 +420,13 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(kdst + dst_off), "l"(kcol + off) : "memory");
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(vdst + dst_off), "l"(vcol + off) : "memory");
               };
-              if (tile_whole<MODE>(p, view, t * kTile)) {
+              if (tile_whole<MODE, GATHER>(p, view, t * kTile)) {
 #pragma unroll
                 for (int r = 0; r < kRounds; ++r) copy(r);
               } else {
 #pragma unroll
                 for (int r = 0; r < kRounds; ++r)
-                  if (group_lives<MODE>(p, view, t * kTile + ((r * kRowsPerRound + r_in) & ~15))) copy(r);
+                  if (group_lives<MODE, GATHER>(p, view, t * kTile + ((r * kRowsPerRound + r_in) & ~15))) copy(r);
               }
               asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full_bar[stage])) : "memory");
               if (++stage == kStages) { stage = 0; phase ^= 1; }
@@ -436,11 +461,13 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const int r0 = lane >> 2, c2 = (lane & 3) * 2;
   const uint32_t stages_u32 = smem_u32(stages);
   float* my_merge = merge + warp * Plan::kMergeFloats;
-  const int slot_floats = Plan::kMergeFloats;
+  const int slot_floats = Plan::kSlotFloats;
 
   constexpr int kColsPerThread = kRowsMax * D / kCThreads;  // 16 (D=128) or 8 (D=64)
   constexpr int kThreadsPerRow = kCThreads / kRowsMax;      // 8
-  const int mrow = ctid / kThreadsPerRow, mcol = (ctid % kThreadsPerRow) * kColsPerThread;
+  // a thread's columns of its row: four from mcol on, and from mcol + 32, mcol + 64 ... on
+  const int mrow = ctid / kThreadsPerRow, mcol = (ctid % kThreadsPerRow) * 4;
+  constexpr int kQuads = kColsPerThread / 4;
   // Writes one row's columns of a thread: `of` relative to the maximum Mf, with the sum Lf.
   auto store_final = [&](int b, int h, int blk, int rows_here, float Mf, float Lf, float* of) {
     if (mrow >= rows_here) return;
@@ -452,21 +479,15 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         const float fa = fast_exp2(Mf - Mu), fb = fast_exp2(Mp - Mu);
         Lf = fa * Lf + fb * Lp;
 #pragma unroll
-        for (int c = 0; c < kColsPerThread; ++c) of[c] = fa * of[c] + fb * merge[mrow * D + mcol + c];
+        for (int c = 0; c < kColsPerThread; ++c) of[c] = fa * of[c] + fb * merge[mrow * D + mcol + (c >> 2) * 32 + (c & 3)];
         Mf = Mn;
       }
     }
     const float inv = Lf > 0.f ? 1.f / Lf : 0.f;
     T* dst = outp + row * D + mcol;
 #pragma unroll
-    for (int c = 0; c < kColsPerThread; c += 8) {
-      uint4 pk;
-      pk.x = pack2<T>(of[c] * inv, of[c + 1] * inv);
-      pk.y = pack2<T>(of[c + 2] * inv, of[c + 3] * inv);
-      pk.z = pack2<T>(of[c + 4] * inv, of[c + 5] * inv);
-      pk.w = pack2<T>(of[c + 6] * inv, of[c + 7] * inv);
-      *reinterpret_cast<uint4*>(dst + c) = pk;
-    }
+    for (int k = 0; k < kQuads; ++k)
+      *reinterpret_cast<uint2*>(dst + 32 * k) = make_uint2(pack2<T>(of[4 * k] * inv, of[4 * k + 1] * inv), pack2<T>(of[4 * k + 2] * inv, of[4 * k + 3] * inv));
     if (p.lse && mcol == 0) p.lse[row] = Lf > 0.f ? Mf + fast_log2(Lf) : -INFINITY;
   };
   // kSuffix, all consumer threads: the partials of the prefix for an item's rows, summed into the merge buffer (rows of
@@ -529,7 +550,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const Piece pc = walker.at(u, u1);
     if (pc.count == 0) break;  // the share ends in front of the next item's tiles
     const int h = pc.hv / p.vblk, blk = pc.hv - h * p.vblk;
-    const ItemView view = item_view<MODE>(p, pc.b);
+    const ItemView view = item_view<MODE, GATHER>(p, MODE != kPlain ? V[pc.b] : item_valid_len(p, pc.b));
     const int valid = view.valid;
     const int rows_here = min(kRowsMax, p.rows - blk * kRowsMax);
     const size_t row_base = (static_cast<size_t>(pc.b) * p.hkv + h) * p.rows + blk * kRowsMax;
@@ -645,7 +666,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     // weights mode: 274 us a tile at a time with a rescale each, see the figures at the entry points.)
     if constexpr (MODE != kPlain) {
       const int mi = lane >> 3, rr = lane & 7;
-      auto takes_part = [&](int tok) { return tok < valid && (MODE != kWindow || tok >= view.lo || tok < p.sinks); };
+      auto takes_part = [&](int tok) { return token_lives<MODE, GATHER>(p, view, tok); };
       auto step = [&](int ti, auto tiles, auto edge) {
         constexpr int N = decltype(tiles)::value;
         constexpr bool EDGE = decltype(edge)::value;  // some of the tokens may not take part
@@ -656,7 +677,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll
         for (int u = 0; u < N; ++u) {
           tok0[u] = view.tile(ti + u) * kTile + ws * 16;
-          if (EDGE) some = tok0[u] < valid && (MODE != kWindow || tok0[u] + 15 >= view.lo || tok0[u] < p.sinks);
+          if (EDGE) some = group_lives<MODE, GATHER>(p, view, tok0[u]);
           kbase[u] = stages_u32 + stage * Plan::kStageBytes;
           freed[u] = &empty_bar[stage];
           mbar_wait(&full_bar[stage], phase, p.status, kFaultFullBarrier);
@@ -780,8 +801,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           if (lane == 0) mbar_arrive(freed[u]);
       };
       auto whole = [&](int ti) {  // every token of the tile takes part (the same for the four warps)
-        const int tok = view.tile(ti) * kTile;
-        return tok + kTile <= valid && (MODE != kWindow || tok >= view.lo || tok + kTile <= p.sinks);
+        return tile_whole<MODE, GATHER>(p, view, view.tile(ti) * kTile);
       };
       for (int ti = pc.tile0; ti < pc.tile0 + pc.count;) {
         if (ti + 1 < pc.tile0 + pc.count && whole(ti) && whole(ti + 1)) {
@@ -801,14 +821,14 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     l_run[1] += __shfl_xor_sync(0xffffffffu, l_run[1], 2);
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
-      *reinterpret_cast<float2*>(my_merge + r0 * D + n * 8 + c2) = make_float2(acc[n][0], acc[n][1]);
-      *reinterpret_cast<float2*>(my_merge + (r0 + 8) * D + n * 8 + c2) = make_float2(acc[n][2], acc[n][3]);
+      *reinterpret_cast<float2*>(my_merge + r0 * Plan::kMergePitch + n * 8 + c2) = make_float2(acc[n][0], acc[n][1]);
+      *reinterpret_cast<float2*>(my_merge + (r0 + 8) * Plan::kMergePitch + n * 8 + c2) = make_float2(acc[n][2], acc[n][3]);
     }
     if ((lane & 3) == 0) {
-      my_merge[kRowsMax * D + r0] = m_run[0];
-      my_merge[kRowsMax * D + r0 + 8] = m_run[1];
-      my_merge[kRowsMax * D + kRowsMax + r0] = l_run[0];
-      my_merge[kRowsMax * D + kRowsMax + r0 + 8] = l_run[1];
+      my_merge[kRowsMax * Plan::kMergePitch + r0] = m_run[0];
+      my_merge[kRowsMax * Plan::kMergePitch + r0 + 8] = m_run[1];
+      my_merge[kRowsMax * Plan::kMergePitch + kRowsMax + r0] = l_run[0];
+      my_merge[kRowsMax * Plan::kMergePitch + kRowsMax + r0 + 8] = l_run[1];
     }
     named_bar_sync(1, kCThreads);
 
@@ -817,7 +837,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       float mw[kConsumerWarps];
 #pragma unroll
       for (int w = 0; w < kConsumerWarps; ++w) {
-        mw[w] = merge[w * Plan::kMergeFloats + kRowsMax * D + mrow];
+        mw[w] = merge[w * Plan::kMergeFloats + kRowsMax * Plan::kMergePitch + mrow];
         M = fmaxf(M, mw[w]);
       }
       const float Mu = M == -INFINITY ? 0.f : M;
@@ -826,11 +846,11 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll
       for (int w = 0; w < kConsumerWarps; ++w) {
         const float cf = fast_exp2(mw[w] - Mu);
-        L += cf * merge[w * Plan::kMergeFloats + kRowsMax * D + kRowsMax + mrow];
-        const float* src = merge + w * Plan::kMergeFloats + mrow * D + mcol;
+        L += cf * merge[w * Plan::kMergeFloats + kRowsMax * Plan::kMergePitch + kRowsMax + mrow];
+        const float* src = merge + w * Plan::kMergeFloats + mrow * Plan::kMergePitch + mcol;
 #pragma unroll
         for (int c = 0; c < kColsPerThread; c += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(src + c);
+          const float4 x = *reinterpret_cast<const float4*>(src + 8 * c);
           o[c] += cf * x.x;
           o[c + 1] += cf * x.y;
           o[c + 2] += cf * x.z;
@@ -850,7 +870,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       if (mrow < rows_here) {
 #pragma unroll
         for (int c = 0; c < kColsPerThread; c += 4)
-          *reinterpret_cast<float4*>(slot + mrow * D + mcol + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+          *reinterpret_cast<float4*>(slot + mrow * D + mcol + 8 * c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
         if (mcol == 0) {
           slot[kRowsMax * D + mrow] = M;
           slot[kRowsMax * D + kRowsMax + mrow] = L;
@@ -884,7 +904,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
               mi_[g] = __ldcg(src + kRowsMax * D + mrow);
               li_[g] = __ldcg(src + kRowsMax * D + kRowsMax + mrow);
 #pragma unroll
-              for (int c = 0; c < kVec; ++c) x[g][c] = __ldcg(reinterpret_cast<const float4*>(src + mrow * D + mcol + 4 * c));
+              for (int c = 0; c < kVec; ++c) x[g][c] = __ldcg(reinterpret_cast<const float4*>(src + mrow * D + mcol + 32 * c));
             }
 #pragma unroll
             for (int g = 0; g < kGroup; ++g) {
@@ -994,9 +1014,9 @@ int plan_decode(const cb200_attn_decode_args* a, DecodeSetup* s, bool need_maps,
   int grid = sms;
   if (a->max_ctas > 0 && a->max_ctas < grid) grid = a->max_ctas;
   // The workspace is sized for a full grid so that one allocation serves every launch.
-  const int fixed = D == 128 ? (s->gather ? SmemPlan<128, true>::kFixedBytes : SmemPlan<128, false>::kFixedBytes)
-                             : (s->gather ? SmemPlan<64, true>::kFixedBytes : SmemPlan<64, false>::kFixedBytes);
-  s->smem_bytes = fixed + (paged ? (a->batch + 1) * 4 : 0) + 1024 + 16;
+  const int fixed = modes ? (D == 128 ? SmemPlan<128, false, kWindow>::kFixedBytes : SmemPlan<64, false, kWindow>::kFixedBytes)
+                          : (D == 128 ? SmemPlan<128, false, kPlain>::kFixedBytes : SmemPlan<64, false, kPlain>::kFixedBytes);
+  s->smem_bytes = fixed + (paged ? (a->batch + 1 + (modes ? a->batch : 0)) * 4 : 0) + 1024 + 16;
   if (s->smem_bytes > 227 * 1024) return CB200_ERR_UNSUPPORTED;  // too many requests for one launch
   // Layout: header | partial slots (two per SM, sized for head_dim 128) | arrival counters.
   // The counters sit at an offset that does not depend on the problem shape: launches of
@@ -1072,7 +1092,7 @@ int launch_decode(const DecodeSetup& s, cudaStream_t stream) {
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(s.grid, 1, 1);
-  cfg.blockDim = dim3(SmemPlan<D, GATHER>::kThreads, 1, 1);
+  cfg.blockDim = dim3(SmemPlan<D, GATHER, MODE>::kThreads, 1, 1);
   cfg.dynamicSmemBytes = s.smem_bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

@@ -7,34 +7,41 @@ namespace cb200 {
 namespace {
 
 // weight_sums[b, h, j] += sum over the kv head's query heads g of 2^(x_gj - lse_g), x the score of the decode kernel in
-// log2 units: the softmax weight that key j had in this step. One thread per four keys of a (request, kv head) and
-// one pass over its score rows; a sum has one owner and its heads are added in their order, so the result does not
-// depend on the launch. Bound by the stream of scores (written a moment ago, partly still in L2) and sums.
-constexpr int kSumThreads = 256;
+// log2 units: the softmax weight that key j had in this step. A thread takes four keys of a (request, kv head), a block
+// apart, and a few heads at a time: every load is a warp's run of 128 bytes, and up to sixteen are in flight. A sum has
+// one owner and its heads are added in their order, so the result does not depend on the launch. Bound by the stream of
+// scores (written a moment ago, partly still in L2) and sums.
+constexpr int kSumThreads = 256, kSumKeys = 4;
 
 __global__ void __launch_bounds__(kSumThreads) weight_sum_kernel(const DecodeParams p, float* __restrict__ sums) {
   pdl_wait();
   const int pair = blockIdx.y, b = pair / p.hkv;
   const int n = min(item_valid_len(p, b), p.raw_len);
-  const int j = (blockIdx.x * kSumThreads + threadIdx.x) * 4;
-  if (j >= n) return;
+  const long long j0 = static_cast<long long>(blockIdx.x) * (kSumThreads * kSumKeys) + threadIdx.x;
+  if (j0 >= n) return;
+  const int j = static_cast<int>(j0), keys = min((n - j + kSumThreads - 1) / kSumThreads, kSumKeys);
   const size_t row = static_cast<size_t>(pair) * p.rows;
   const float* x = p.raw + row * p.raw_pitch + j;
   const float* lse = p.lse + row;
-  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  float* dst = sums + static_cast<size_t>(pair) * p.raw_len + j;
+  float old[kSumKeys], w[kSumKeys];
+#pragma unroll
+  for (int i = 0; i < kSumKeys; ++i) {
+    old[i] = i < keys ? dst[i * kSumThreads] : 0.f;
+    w[i] = 0.f;
+  }
 #pragma unroll 4
   for (int g = 0; g < p.rows; ++g) {
-    const float4 v = *reinterpret_cast<const float4*>(x + g * p.raw_pitch);  // pitch and start: multiples of 4
     const float l = __ldg(lse + g);
-    w[0] += exp2f(v.x - l);
-    w[1] += exp2f(v.y - l);
-    w[2] += exp2f(v.z - l);
-    w[3] += exp2f(v.w - l);
-  }
-  float* dst = sums + static_cast<size_t>(pair) * p.raw_len + j;
+    float v[kSumKeys];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (j + i < n) dst[i] += w[i];
+    for (int i = 0; i < kSumKeys; ++i) v[i] = i < keys ? __ldcs(x + g * p.raw_pitch + i * kSumThreads) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kSumKeys; ++i) w[i] += exp2f(v[i] - l);
+  }
+#pragma unroll
+  for (int i = 0; i < kSumKeys; ++i)
+    if (i < keys) dst[i * kSumThreads] = old[i] + w[i];
 }
 
 // floats between the score rows of two query heads: whole 32-byte runs
@@ -79,7 +86,7 @@ extern "C" int cb200_attn_decode_weights(const cb200_attn_decode_args* a, float*
   const int done = launch_decode_mode<kWeights>(s, a, st);
   if (done != CB200_OK) return done;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((max_len + 4LL * kSumThreads - 1) / (4 * kSumThreads)), static_cast<unsigned>(pairs), 1);
+  cfg.gridDim = dim3(static_cast<unsigned>((max_len + static_cast<long long>(kSumKeys) * kSumThreads - 1) / (kSumKeys * kSumThreads)), static_cast<unsigned>(pairs), 1);
   cfg.blockDim = dim3(kSumThreads, 1, 1);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
