@@ -260,10 +260,11 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   if (warp >= kConsumerWarps) {
     // ================================================================= producer warp(s)
     int stage = 0, phase = 0;
+    Piece pc{};
     for (int u = u0; u < u1;) {
-      const Piece pc = walker.at(u, u1);
+      pc = MODE == kPlain || u == u0 ? walker.at(u, u1) : walker.after(pc, u, u1);
       if (pc.count == 0) break;  // the share ends in front of the next item's tiles
-      const int h = pc.hv / p.vblk;
+      const int h = MODE != kPlain && p.vblk == 1 ? pc.hv : pc.hv / p.vblk;
       const ItemView view = item_view<MODE, GATHER>(p, MODE != kPlain ? V[pc.b] : item_valid_len(p, pc.b));
       const int valid = view.valid;
       const int page_base = p.paged ? p.kv_indptr[pc.b] : 0;
@@ -546,10 +547,11 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   };
 
   int stage = 0, phase = 0;
+  Piece pc{};
   for (int u = u0; u < u1;) {
-    const Piece pc = walker.at(u, u1);
+    pc = MODE == kPlain || u == u0 ? walker.at(u, u1) : walker.after(pc, u, u1);
     if (pc.count == 0) break;  // the share ends in front of the next item's tiles
-    const int h = pc.hv / p.vblk, blk = pc.hv - h * p.vblk;
+    const int h = MODE != kPlain && p.vblk == 1 ? pc.hv : pc.hv / p.vblk, blk = pc.hv - h * p.vblk;
     const ItemView view = item_view<MODE, GATHER>(p, MODE != kPlain ? V[pc.b] : item_valid_len(p, pc.b));
     const int valid = view.valid;
     const int rows_here = min(kRowsMax, p.rows - blk * kRowsMax);
