@@ -6,9 +6,9 @@
 // their order, into the destination pages, and their sums with them.
 //
 // Two kernels. evict_select_kernel (one CTA per (request, kv head)) finds the smallest kept sum with two or three
-// histograms over the sums, which it holds in registers, and writes the kept indices in order. evict_copy_kernel moves the rows: it has no dependence between
-// its CTAs (source and destination pages are disjoint), so it is a plain gather of 2 D-byte rows that is bound by the
-// memory's bandwidth, which is nearly all of the operator's time where the cache is large.
+// histograms over the sums, which it holds in registers, and writes the kept indices in order. evict_copy_kernel moves the
+// rows: it has no dependence between its CTAs (source and destination pages are disjoint), so it is a plain gather of
+// 2 D-byte rows that is bound by the memory's bandwidth, which is nearly all of the operator's time where the cache is large.
 
 #include "common.cuh"
 
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kSelThreads, KEYS <= 16 ? 2 : 1) evict_select_
       break;
     }
     base = low;
-    top = min(top, low + ((1u << shift) - 1));
+    top = low + min(top - low, (1u << shift) - 1);  // the bin's end may lie behind the last 32-bit number
   }
 
   // ---- keys above the threshold stay, and the first `ties` of those equal to it. Where a kept token goes follows from how
@@ -308,8 +308,10 @@ extern "C" int cb200_kv_evict(const cb200_kv_evict_args* a, void* stream) {
     return CB200_ERR_BAD_ARG;
   if (static_cast<long long>(a->sinks) + a->recent > a->budget) return CB200_ERR_BAD_ARG;
   if (a->head_dim % 8 || a->batch > 65535) return CB200_ERR_UNSUPPORTED;
-  // token counts are held in 32 bits
-  if (static_cast<long long>(a->num_kv_indices) * a->page_size >= (1LL << 31)) return CB200_ERR_UNSUPPORTED;
+  // token counts, and places up to a few blocks of threads behind them, are held in 32 bits
+  constexpr long long kMost = 1LL << 30;
+  if (static_cast<long long>(a->num_kv_indices) * a->page_size > kMost || a->max_len > kMost || a->budget > kMost || a->head_dim > 65536)
+    return CB200_ERR_UNSUPPORTED;
   // Small CTAs where the rows would not give every SM several large ones (one request of 512 tokens and 8 heads).
   const long long rows = static_cast<long long>(a->budget) * a->num_kv_heads;
   const int copy_rows = rows * a->batch >= 128LL * 4 * 148 ? 128 : 32;

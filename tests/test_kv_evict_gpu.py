@@ -124,6 +124,15 @@ def test_ties_and_special_values(kind):
     Case(lens, hkv, 64, 16, torch.bfloat16, 100, sums=s, seed=4).check(3, 10)
 
 
+@pytest.mark.parametrize("nans", [5, 87, 88, 150])
+def test_more_nans_than_stay(nans):
+    """The keys then span the whole 32-bit range, and the range of the last histogram ends at its last number."""
+    s = torch.rand(2, 2, 300, generator=torch.Generator().manual_seed(17))
+    s[..., 0:20], s[..., 20:60] = math.inf, -math.inf
+    s[..., 100:100 + nans] = math.nan
+    Case([300, 260], 2, 64, 16, torch.bfloat16, 100, sums=s, seed=4).check(3, 10)
+
+
 @pytest.mark.parametrize("max_len", [1, 50, 129, 600])
 def test_tokens_without_a_record_weigh_nothing(max_len):
     Case([513, 130, 4], 2, 64, 16, torch.bfloat16, 100, max_len=max_len, seed=5).check(4, 20)
