@@ -221,7 +221,8 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   pdl_wait();
   pdl_launch_dependents();
 
-  // ---- the work list
+  // ---- the work list. Row offsets are caller data: clipped to the rows there are, so no row outside `out` is written.
+  auto q_row = [&](int r) { return min(max(__ldg(p.qo_indptr + r), 0), p.total_q); };
   int pre_lo = 0, pre_hi = 0, pre_klo = 0, pre_khi = 0;  // the ranges of the first 32 requests (lane = request)
   const bool heads_pair = (p.hq / p.hkv) % 2 == 0;  // the blocks are two heads; otherwise two query tiles
   const int unit = heads_pair ? kBM : 2 * kBM;                 // query rows of a request that an item covers
@@ -229,21 +230,21 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   int q_units;
   {
     if (lane < p.batch) {
-      pre_lo = __ldg(p.qo_indptr + lane);
-      pre_hi = __ldg(p.qo_indptr + lane + 1);
+      pre_lo = q_row(lane);
+      pre_hi = q_row(lane + 1);
       pre_klo = __ldg(p.kv_indptr + lane);
       pre_khi = __ldg(p.kv_indptr + lane + 1);
     }
     int mine = pre_hi > pre_lo ? ceil_div(pre_hi - pre_lo, unit) : 0;
 #pragma unroll 4
     for (int r = 32 + lane; r < p.batch; r += 32) {
-      const int lo = __ldg(p.qo_indptr + r), hi = __ldg(p.qo_indptr + r + 1);
+      const int lo = q_row(r), hi = q_row(r + 1);
       mine += hi > lo ? ceil_div(hi - lo, unit) : 0;
     }
     q_units = __reduce_add_sync(0xffffffffu, mine);
     // rows in front of the first request and behind the last, shared out over the grid
     if (p.fill) {
-      const int head = min(max(__ldg(p.qo_indptr), 0), p.total_q), rest = min(max(__ldg(p.qo_indptr + p.batch), head), p.total_q);
+      const int head = q_row(0), rest = max(q_row(p.batch), head);
       const long long none = head + (p.total_q - rest), step = static_cast<long long>(gridDim.x) * blockDim.x;
       const long long i0 = static_cast<long long>(blockIdx.x) * blockDim.x + tid;
       auto row_of = [&](long long r) { return static_cast<size_t>(r < head ? r : r - head + rest); };
@@ -270,8 +271,8 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       const int rr = r0 + lane;
       int lo = pre_lo, hi = pre_hi, klo = pre_klo, khi = pre_khi;
       if (r0 > 0) {
-        lo = rr < p.batch ? __ldg(p.qo_indptr + rr) : 0;
-        hi = rr < p.batch ? __ldg(p.qo_indptr + rr + 1) : 0;
+        lo = rr < p.batch ? q_row(rr) : 0;
+        hi = rr < p.batch ? q_row(rr + 1) : 0;
         klo = rr < p.batch ? __ldg(p.kv_indptr + rr) : 0;
         khi = rr < p.batch ? __ldg(p.kv_indptr + rr + 1) : 0;
       }
@@ -764,6 +765,10 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                            pack2<T>(v[i + 12] * inv, v[i + 13] * inv), pack2<T>(v[i + 14] * inv, v[i + 15] * inv));
         }
       }
+      if (live_row && l_run == 0.f) {  // no key seen: what the tile's other rows see may hold Inf, and 0 * Inf is in O
+#pragma unroll 1
+        for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + orow * D)[i] = make_uint4(0u, 0u, 0u, 0u);
+      }
       if (live_row && p.lse) p.lse[orow] = l_run > 0.f ? m_ref + fast_log2(l_run) : -INFINITY;
     }
   }
@@ -785,7 +790,16 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
 template <typename T, int D, bool PAGED>
 int launch_kernel(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const Params& p, long long items, cudaStream_t stream) {
   auto kern = window_prefill_kernel<T, D, PAGED>;
-  CB200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmemBytes));
+  static bool ready[16] = {false};  // per device
+  int dev = 0;
+  CB200_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 16 || !ready[dev]) {
+    cudaFuncAttributes attr;
+    CB200_CUDA_TRY(cudaFuncGetAttributes(&attr, kern));
+    if (attr.numRegs < Roles<PAGED>::kRegsLaunch) return CB200_ERR_UNSUPPORTED;  // the softmax warps would wait for registers for good
+    CB200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmemBytes));
+    if (dev < 16) ready[dev] = true;
+  }
   const int sms = sm_count();
   if (sms <= 0) return CB200_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
@@ -811,6 +825,7 @@ int check_window(const cb200_attn_prefill_ragged_args* a) {
   if (a->head_dim != 64 && a->head_dim != 128) return CB200_ERR_UNSUPPORTED;
   if (a->dtype != CB200_F16 && a->dtype != CB200_BF16) return CB200_ERR_UNSUPPORTED;
   if (static_cast<long long>(a->num_qo_heads) * (ceil_div(a->total_q, kBM) + a->batch) >= (1LL << 31)) return CB200_ERR_UNSUPPORTED;
+  if (a->total_q > (1 << 30) || (a->kv_indices ? a->num_kv_indices : a->total_kv) > (1 << 30)) return CB200_ERR_UNSUPPORTED;  // rows and keys, rounded up to tiles, in 32 bits
   if (!a->q || !a->k || !a->v || !a->out || !a->qo_indptr || !a->kv_indptr) return CB200_ERR_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v) |
        reinterpret_cast<uintptr_t>(a->out)) & 15)

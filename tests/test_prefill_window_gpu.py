@@ -142,6 +142,27 @@ def test_isolation_of_neighbours(paged):
     check(out[rows.cuda()], lse[rows.cuda()], want[rows], want_lse[rows], spread[rows], c.dtype, one_p=True)
 
 
+@PAGED
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_rows_in_front_of_the_keys_are_empty_whatever_the_others_see(paged, value):
+    """20 rows over 5 keys: the first 15 see none of them."""
+    c = Case([(20, 5)], 4, 2, 128, torch.bfloat16, 3, 0, paged, seed=40)
+    c.v[:5] = value
+    out, lse = c.run()
+    assert (out[:15] == 0).all() and (lse[:15] == -math.inf).all() and (lse[15:] > -math.inf).all()
+
+
+@PAGED
+def test_row_offsets_behind_the_rows_are_clipped(paged):
+    c = Case([(30, 30), (40, 60)], 4, 2, 64, torch.bfloat16, 20, 2, paged, seed=41)
+    args = c.args()
+    want, want_lse = c.call(*args)
+    args[0] = torch.cat([args[0], args[0][:1]])[:70]
+    args[3] = torch.tensor([0, 30, 2000], dtype=torch.int32, device="cuda")
+    out, lse = c.call(*args)
+    assert torch.equal(out[:30], want[:30]) and torch.equal(lse[:30], want_lse[:30])
+
+
 def test_pages_of_unseen_keys_may_be_gone():
     c = Case([(70, 900), (5, 300)], 4, 2, 128, torch.bfloat16, 100, 3, True, seed=8)
     args = c.args()
