@@ -665,7 +665,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     // (a request's last tile, the edges of a window): with 32 tokens in hand the two chains of score MMAs overlap, and
     // the reductions of the maximum cost half as much a token. O is rescaled only when a maximum has grown, which
     // after the first tiles is rare; the factor would be exactly 1. (64 requests of 512..8192 tokens in 16-token pages,
-    // weights mode: 274 us a tile at a time with a rescale each, see the figures at the entry points.)
+    // weights mode: 274 us a tile at a time with a rescale each, 248 so.)
     if constexpr (MODE != kPlain) {
       const int mi = lane >> 3, rr = lane & 7;
       auto takes_part = [&](int tok) { return token_lives<MODE, GATHER>(p, view, tok); };
@@ -1009,8 +1009,11 @@ int plan_decode(const cb200_attn_decode_args* a, DecodeSetup* s, bool need_maps,
   const long long tiles_max = paged ? static_cast<long long>(a->batch) * ((static_cast<long long>(a->num_kv_indices) * a->page_size + kTile - 1) / kTile + 1 + kPieceUnits)
                                     : tiles_ub;
   if (tiles_max * p.hkv * p.vblk >= (1LL << 31)) return CB200_ERR_UNSUPPORTED;
-  // the modes hold a token's place in the pool in 32 bits (2^31 tokens would be 256 GB of the narrowest rows)
-  if (modes && static_cast<long long>(a->num_pages) * a->page_size >= (1LL << 31)) return CB200_ERR_UNSUPPORTED;
+  // the modes hold a token's place in the pool in 32 bits (2^31 tokens would be 256 GB of the narrowest rows), and its
+  // place in its request, rounded up to whole tiles, with a sign
+  if (modes && paged && (static_cast<long long>(a->num_pages) * a->page_size >= (1LL << 31) ||
+                         static_cast<long long>(a->num_kv_indices) * a->page_size > (1LL << 30)))
+    return CB200_ERR_UNSUPPORTED;
   const int sms = sm_count();
   if (sms <= 0) return CB200_ERR_CUDA;
   int grid = sms;

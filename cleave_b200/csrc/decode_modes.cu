@@ -10,7 +10,7 @@ namespace {
 // log2 units: the softmax weight that key j had in this step. A thread takes four keys of a (request, kv head), a block
 // apart, and a few heads at a time: every load is a warp's run of 128 bytes, and up to sixteen are in flight. A sum has
 // one owner and its heads are added in their order, so the result does not depend on the launch. Bound by the stream of
-// scores (written a moment ago, partly still in L2) and sums.
+// scores (written a moment ago, partly still in L2) and sums. A row whose scores are all -inf has no weights: it adds nothing.
 constexpr int kSumThreads = 256, kSumKeys = 4;
 
 __global__ void __launch_bounds__(kSumThreads) weight_sum_kernel(const DecodeParams p, float* __restrict__ sums) {
@@ -32,7 +32,8 @@ __global__ void __launch_bounds__(kSumThreads) weight_sum_kernel(const DecodePar
   }
 #pragma unroll 4
   for (int g = 0; g < p.rows; ++g) {
-    const float l = __ldg(lse + g);
+    float l = __ldg(lse + g);
+    if (l == -INFINITY) l = INFINITY;
     float v[kSumKeys];
 #pragma unroll
     for (int i = 0; i < kSumKeys; ++i) v[i] = i < keys ? __ldcs(x + g * p.raw_pitch + i * kSumThreads) : -INFINITY;

@@ -160,6 +160,16 @@ def test_weights_cut_over_ctas(max_ctas):
     _check_weights(Paged([5000, 1, 300, 4097], 8, 2, 128, 64, torch.float16, seed=32), 5000, max_ctas=max_ctas)
 
 
+def test_rows_without_a_finite_score_add_nothing():
+    c = Paged([70, 40], 4, 2, 64, 16, torch.bfloat16, seed=31)
+    c.q.abs_().add_(0.5)
+    for t in range(40):
+        c.poison(1, [t], -math.inf)
+    sums = torch.full((2, 2, 70), 0.25, device="cuda")
+    _ops().gqa_paged_decode_weights(*c.args(), sums)
+    assert (sums[1] == 0.25).all() and (sums[0] > 0.25).all()
+
+
 def test_weights_add_up_to_the_query_heads():
     c = Paged([700, 1, 64], 8, 2, 128, 64, torch.bfloat16, seed=33)
     sums = torch.zeros(3, 2, 704, device="cuda")
