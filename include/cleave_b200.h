@@ -168,7 +168,8 @@ int cb200_attn_decode_shared_prefix(const cb200_attn_decode_args* a, const int32
  *   kept              (batch, num_kv_heads, budget): the indices that stay, ascending, then -1
  *   kept_sums         (batch, num_kv_heads, max_len): their sums, then 0; must not overlap weight_sums
  *   dst_last_page_len (batch): tokens in the last destination page, 0 for B = 0
- * sinks + recent <= budget, head_dim a multiple of 8, 16-bit elements of either type, batch <= 65535. Page tables are not
+ * sinks + recent <= budget, head_dim a multiple of 8, 16-bit elements of either type, batch <= 65535; budget, max_len and
+ * the tokens of the page table <= 2^30. Page tables are not
  * trusted: ranges are clipped to the tables, source pages to the pool, and rows whose destination page does not exist
  * are not written. Two kernels, no workspace. No counterpart in the reference.
  * ---------------------------------------------------------------------------------------- */
@@ -406,7 +407,9 @@ int cb200_attn_prefill_ragged(const cb200_attn_prefill_ragged_args* a, void* str
  * rows hold; page ids of such keys may name pages that belong to others. fill, bit 0: rows of `out` that belong to no
  * request (in front of the first or behind the last) become 0, bit 1: those of `lse` become -inf; without the bit they
  * stay as they are. Arguments, workspace
- * (cb200_attn_prefill_ragged_workspace_bytes) and results otherwise as above. No counterpart in the reference. */
+ * (cb200_attn_prefill_ragged_workspace_bytes) and results otherwise as above. A row of V that some query of a request sees should be finite: where another
+ * query of the request does not see it, its weight there is 0, and 0 * Inf is not. At most 2^30 rows of Q and keys. No
+ * counterpart in the reference. */
 int cb200_attn_prefill_ragged_window(const cb200_attn_prefill_ragged_args* a, int window, int sinks, int fill, void* stream);
 
 /* ------------------------------------------------------------------------------------------
