@@ -546,32 +546,43 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     named_bar_sync(1, kCThreads);
   };
 
+  // Q fragments (A operand) of a piece's rows; those beyond its last are zero
+  uint32_t qf[D / 16][4];
+  auto load_q = [&](const Piece& piece) {
+    const int h = MODE != kPlain && p.vblk == 1 ? piece.hv : piece.hv / p.vblk, blk = piece.hv - h * p.vblk;
+    const int rows_here = min(kRowsMax, p.rows - blk * kRowsMax);
+    const size_t row_base = (static_cast<size_t>(piece.b) * p.hkv + h) * p.rows + blk * kRowsMax;
+    const T* qrow0 = reinterpret_cast<const T*>(p.q) + (row_base + r0) * D;
+    const T* qrow1 = qrow0 + 8 * D;
+    const bool ok0 = r0 < rows_here, ok1 = r0 + 8 < rows_here;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const int d = kk * 16 + c2;
+      qf[kk][0] = ok0 ? *reinterpret_cast<const uint32_t*>(qrow0 + d) : 0u;
+      qf[kk][1] = ok1 ? *reinterpret_cast<const uint32_t*>(qrow1 + d) : 0u;
+      qf[kk][2] = ok0 ? *reinterpret_cast<const uint32_t*>(qrow0 + d + 8) : 0u;
+      qf[kk][3] = ok1 ? *reinterpret_cast<const uint32_t*>(qrow1 + d + 8) : 0u;
+    }
+  };
+
   int stage = 0, phase = 0;
-  Piece pc{};
-  for (int u = u0; u < u1;) {
-    pc = MODE == kPlain || u == u0 ? walker.at(u, u1) : walker.after(pc, u, u1);
+  Piece pc{}, next{};
+  int u_next = u0;
+  for (int u = u0; u < u1; u = u_next) {
+    if (MODE == kPlain || u == u0) {
+      pc = walker.at(u, u1);
+      if (pc.count > 0) load_q(pc);
+    } else {
+      pc = next;
+    }
     if (pc.count == 0) break;  // the share ends in front of the next item's tiles
+    u_next = u + pc.count;
     const int h = MODE != kPlain && p.vblk == 1 ? pc.hv : pc.hv / p.vblk, blk = pc.hv - h * p.vblk;
     const ItemView view = item_view<MODE, GATHER>(p, MODE != kPlain ? V[pc.b] : item_valid_len(p, pc.b));
     const int valid = view.valid;
     const int rows_here = min(kRowsMax, p.rows - blk * kRowsMax);
     const size_t row_base = (static_cast<size_t>(pc.b) * p.hkv + h) * p.rows + blk * kRowsMax;
 
-    // ---- Q fragments (A operand), rows beyond rows_here are zero
-    uint32_t qf[D / 16][4];
-    {
-      const T* qrow0 = reinterpret_cast<const T*>(p.q) + (row_base + r0) * D;
-      const T* qrow1 = qrow0 + 8 * D;
-      const bool ok0 = r0 < rows_here, ok1 = r0 + 8 < rows_here;
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const int d = kk * 16 + c2;
-        qf[kk][0] = ok0 ? *reinterpret_cast<const uint32_t*>(qrow0 + d) : 0u;
-        qf[kk][1] = ok1 ? *reinterpret_cast<const uint32_t*>(qrow1 + d) : 0u;
-        qf[kk][2] = ok0 ? *reinterpret_cast<const uint32_t*>(qrow0 + d + 8) : 0u;
-        qf[kk][3] = ok1 ? *reinterpret_cast<const uint32_t*>(qrow1 + d + 8) : 0u;
-      }
-    }
     float acc[D / 8][4];
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
@@ -816,6 +827,13 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       }
     }
 
+    if constexpr (MODE != kPlain) {
+      // The next piece's rows of Q are on their way while this one's states are merged (128 requests of 100 .. 2048 tokens,
+      // 16-token pages: 108.7 -> 104.2 us)
+      next = walker.after(pc, u_next, u1);
+      if (next.count > 0) load_q(next);
+    }
+
     // ---- merge the four warps' states through shared memory
     l_run[0] += __shfl_xor_sync(0xffffffffu, l_run[0], 1);
     l_run[0] += __shfl_xor_sync(0xffffffffu, l_run[0], 2);
@@ -932,7 +950,6 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       }
     }
     named_bar_sync(1, kCThreads);  // merge buffer and flag are free again
-    u += pc.count;
   }
   if constexpr (MODE == kSuffix) {
     // requests with nothing behind the prefix; their (request, kv head) pairs are shared out over the CTAs
