@@ -8,7 +8,7 @@
  *
  * Conventions
  *  - plain pointers and sizes only; all tensor pointers are DEVICE pointers, caller-owned,
- *    inputs are never written;
+ *    inputs are never written (but the sums and caches that cb200_attn_decode_weights and cb200_kv_evict update in place);
  *  - `stream` is a cudaStream_t passed as void* (NULL = the legacy default stream);
  *  - every launch function returns a cb200_status (0 = ok); nothing throws, nothing
  *    allocates device memory, nothing synchronises: a launch can be captured in a CUDA graph
