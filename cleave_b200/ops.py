@@ -150,11 +150,18 @@ def _raw_stream(index: int) -> int:
 
 
 def _check_all(device, **tensors) -> None:
-    """Refuses tensors that are not contiguous or not on ``device``."""
+    """Refuses tensors that are not contiguous or not on ``device`` (compared by index: comparing device objects costs
+    three times as much)."""
+    index = device.index
     for name, t in tensors.items():
-        if t is not None and (t.device != device or not t.is_contiguous()):
+        if t is not None and (t.get_device() != index or not t.is_contiguous()):
             _cuda(t, name)
             raise ValueError(f"{name} must be on {device}, not on {t.device}")
+
+
+def _empty2(rows, cols, device) -> torch.Tensor:
+    """An uninitialised (rows, cols) float32 tensor (torch.empty takes a microsecond more to do the same)."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=torch.float32, device=device)
 
 
 def _private_workspace(nbytes: int, device) -> torch.Tensor:
@@ -219,7 +226,7 @@ def _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page
     elif out.shape != q.shape or out.dtype != dtype:
         raise ValueError("out must have q's shape, dtype and device")
     if lse is None:
-        lse = torch.empty((batch, hq), dtype=torch.float32, device=device)
+        lse = _empty2(batch, hq, device)
     elif tuple(lse.shape) != (batch, hq) or lse.dtype != torch.float32:
         raise ValueError("lse must be (batch, HQ) float32 on q's device")
     a = _lib.AttnDecodeArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), last,
@@ -351,9 +358,9 @@ def kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last
         raise ValueError("kv_indptr and dst_indptr must have batch + 1 entries")
     if kv_last_page_len is not None and kv_last_page_len.numel() != batch:
         raise ValueError("kv_last_page_len must hold batch values")
-    kept = torch.empty((batch, hkv, budget), dtype=i32, device=device)
+    kept = torch.empty_strided((batch, hkv, budget), (hkv * budget, budget, 1), dtype=i32, device=device)
     sums = torch.empty_like(weight_sums)
-    last = torch.empty(batch, dtype=i32, device=device)
+    last = torch.empty_strided((batch,), (1,), dtype=i32, device=device)
     a = _lib.KvEvictArgs(k_cache.data_ptr(), v_cache.data_ptr(), weight_sums.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(),
                          None if kv_last_page_len is None else kv_last_page_len.data_ptr(), dst_indptr.data_ptr(),
                          dst_indices.data_ptr(), kept.data_ptr(), sums.data_ptr(), last.data_ptr(), batch, hkv, d, page_size,
@@ -563,7 +570,7 @@ def _prefill_window(q, k, v, qo_indptr, kv_indptr, kv_indices, sm_scale, window,
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("out must have q's shape, dtype and device")
     if lse is None:
-        lse = torch.empty((total_q, hq), dtype=torch.float32, device=device)
+        lse = _empty2(total_q, hq, device)
     elif tuple(lse.shape) != (total_q, hq) or lse.dtype != torch.float32:
         raise ValueError("lse must be (total_q, HQ) float32 on q's device")
     paged = kv_indices is not None
