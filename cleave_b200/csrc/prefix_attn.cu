@@ -356,7 +356,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       tc_fence_after();
       float psum = 0.f;
       {
-        uint32_t pk[32];
+        uint32_t pk[32];  // P in the storage type, as the operand of a 16-bit product must be; its sum is that of the fp32 values
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           const int c = 2 * i;
@@ -389,7 +389,9 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       tmem_ld_wait();
       if (live_row) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(dst + c0 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        for (int i = 0; i < 32; i += 8)  // whole sectors: neighbouring lanes write rows that are far apart
+          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + c0 + i), "r"(o[i]), "r"(o[i + 1]), "r"(o[i + 2]),
+                       "r"(o[i + 3]), "r"(o[i + 4]), "r"(o[i + 5]), "r"(o[i + 6]), "r"(o[i + 7]) : "memory");
       }
     }
     if (!half && live_row) {
@@ -423,12 +425,14 @@ int plan_prefix(const cb200_attn_decode_args* a, int prefix_len, Plan* pl) {
   if (sms <= 0) return CB200_ERR_CUDA;
   // Parts per (kv head, row block): the fewest rounds of tiles over the SMs, in units of a tile (about 1.4 us). A CTA
   // costs about three tiles beside its tiles (launch, first loads, the partial); every part adds one fp32 copy of
-  // the rows that is written and read again.
+  // the rows that is written and read again, and every eight parts a round trip to L2 for each (request, kv head) of the
+  // second kernel, of which a CTA has its share one after the other.
   const double merge = 2.0 * a->batch * a->num_qo_heads * a->head_dim * 4 / 6e6 / 1.4;
+  const double trip = 0.8 * a->batch * a->num_kv_heads / sms;
   double best = 0;
   pl->splits = 1;
   for (int s = 1; s <= pl->n_tiles && s <= 256; ++s) {
-    const double cost = static_cast<double>((base * s + sms - 1) / sms) * (ceil_div(pl->n_tiles, s) + 3) + merge * s;
+    const double cost = static_cast<double>((base * s + sms - 1) / sms) * (ceil_div(pl->n_tiles, s) + 3) + merge * s + trip * ceil_div(s, 8);
     if (s == 1 || cost < best) {
       best = cost;
       pl->splits = s;
@@ -516,7 +520,7 @@ extern "C" int cb200_attn_decode_shared_prefix(const cb200_attn_decode_args* a, 
     const int prc = pre::plan_prefix(a, prefix_len, &pl);
     if (prc != CB200_OK) return prc;
     if (!scratch || scratch_bytes < pl.o_bytes + pl.ml_bytes) return CB200_ERR_WORKSPACE;
-    if (reinterpret_cast<uintptr_t>(scratch) & 15) return CB200_ERR_ALIGNMENT;
+    if (reinterpret_cast<uintptr_t>(scratch) & 31) return CB200_ERR_ALIGNMENT;
     pre::Params p{};
     p.indices = prefix_indices;
     p.k = a->k_cache;

@@ -149,7 +149,7 @@ int cb200_attn_decode_weights(const cb200_attn_decode_args* a, float* weight_sum
  * The prefix's keys and values are read once for the batch, on the tcgen05 tensor cores. `out` and `lse` cover both
  * parts; a request with neither gives 0 / -inf. prefix_len = 0 is plain decode (prefix_indices and scratch may then be
  * NULL). num_qo_heads / num_kv_heads <= 128, prefix_len <= 2^30. `scratch`
- * (cb200_attn_decode_shared_prefix_scratch_bytes, 16-byte aligned, any contents; 0 bytes for prefix_len = 0) holds fp32
+ * (cb200_attn_decode_shared_prefix_scratch_bytes, 32-byte aligned, any contents; 0 bytes for prefix_len = 0) holds fp32
  * partials between the two kernels; the workspace is that of cb200_attn_decode. No counterpart in the reference.
  * ---------------------------------------------------------------------------------------- */
 size_t cb200_attn_decode_shared_prefix_scratch_bytes(const cb200_attn_decode_args* a, int prefix_len);
