@@ -79,7 +79,7 @@ extern "C" int cb200_attn_decode_weights(const cb200_attn_decode_args* a, float*
   const long long pairs = static_cast<long long>(a->batch) * a->num_kv_heads;
   if (pairs > 65535) return CB200_ERR_UNSUPPORTED;
   if (!scratch || scratch_bytes < cb200_attn_decode_weights_scratch_bytes(a, max_len)) return CB200_ERR_WORKSPACE;
-  if ((reinterpret_cast<uintptr_t>(scratch) & 31) || (reinterpret_cast<uintptr_t>(weight_sums) & 15)) return CB200_ERR_ALIGNMENT;
+  if ((reinterpret_cast<uintptr_t>(scratch) & 31) || (reinterpret_cast<uintptr_t>(weight_sums) & 3)) return CB200_ERR_ALIGNMENT;
   s.p.raw = static_cast<float*>(scratch);
   s.p.raw_len = max_len;
   s.p.raw_pitch = raw_pitch(max_len);

@@ -134,7 +134,7 @@ int cb200_attn_decode_window(const cb200_attn_decode_args* a, int window, int si
 /* ------------------------------------------------------------------------------------------
  * Decode attention (paged caches) that also accumulates what every key has weighed:
  *   weight_sums[b, h, j] += sum over the query heads of kv head h of softmax weight j     (fp32)
- * weight_sums is (batch, num_kv_heads, max_len), contiguous, 16-byte aligned, updated in place; entries behind a
+ * weight_sums is (batch, num_kv_heads, max_len), contiguous, updated in place; entries behind a
  * request's last token are left as they are, tokens from max_len on are attended but not recorded. Requests may share
  * pages. `lse` must not be NULL. `scratch` (cb200_attn_decode_weights_scratch_bytes, 32-byte aligned, any contents) holds
  * the scores between the two kernels. batch * num_kv_heads <= 65535. No counterpart in the reference.

@@ -160,6 +160,15 @@ def test_weights_cut_over_ctas(max_ctas):
     _check_weights(Paged([5000, 1, 300, 4097], 8, 2, 128, 64, torch.float16, seed=32), 5000, max_ctas=max_ctas)
 
 
+def test_sums_may_start_anywhere():
+    c = Paged([70, 41], 4, 1, 64, 16, torch.bfloat16, seed=32)
+    whole = torch.zeros(3, 1, 71, device="cuda")
+    want = torch.zeros(2, 1, 71, device="cuda")
+    _ops().gqa_paged_decode_weights(*c.args(), whole[1:])
+    _ops().gqa_paged_decode_weights(*c.args(), want)
+    assert torch.equal(whole[1:], want) and (whole[0] == 0).all()
+
+
 def test_rows_without_a_finite_score_add_nothing():
     c = Paged([70, 40], 4, 2, 64, 16, torch.bfloat16, seed=31)
     c.q.abs_().add_(0.5)
