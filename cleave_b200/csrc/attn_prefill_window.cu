@@ -11,7 +11,7 @@
 // Why two: one block is a chain - scores, softmax, value product - in which the tensor cores idle during the softmax and
 // the softmax warps during the products. With two blocks in turn the one's softmax runs beside the other's products, and a
 // CTA asks L2 for half as many keys per row. Measured for one prompt of 8191 tokens, window 1024, 32/8 heads of 128:
-// 203 us where the same tiles on the one-block kernel of the plain prefill take 232; a step of both blocks takes 4200
+// 206 us where the same tiles on the one-block kernel of the plain prefill take 232; a step of both blocks takes 4200
 // cycles, of which the tensor cores work 2050 and the exponentials' unit as much. What remains is latency: a softmax warp
 // has its scheduler nearly to itself while the other block's products run, and issues an exponential every 16
 // cycles where two warps at work issue one every 9.
