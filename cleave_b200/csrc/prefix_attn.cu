@@ -425,12 +425,12 @@ int plan_prefix(const cb200_attn_decode_args* a, int prefix_len, Plan* pl) {
   const long long base = static_cast<long long>(a->num_kv_heads) * pl->blocks;
   const int sms = sm_count();
   if (sms <= 0) return CB200_ERR_CUDA;
-  // Parts per (kv head, row block): the fewest rounds of tiles over the SMs, in units of a tile (about 1.4 us). A CTA
+  // Parts per (kv head, row block): the fewest rounds of tiles over the SMs, in units of a tile (about 1.2 us). A CTA
   // costs about three tiles beside its tiles (launch, first loads, the partial); every part adds one fp32 copy of
   // the rows that is written and read again, and every eight parts a round trip to L2 for each (request, kv head) of the
   // second kernel, of which a CTA has its share one after the other.
-  const double merge = 2.0 * a->batch * a->num_qo_heads * a->head_dim * 4 / 6e6 / 1.4;
-  const double trip = 0.8 * a->batch * a->num_kv_heads / sms;
+  const double merge = 2.0 * a->batch * a->num_qo_heads * a->head_dim * 4 / 6e6 / 1.2;
+  const double trip = 0.95 * a->batch * a->num_kv_heads / sms;
   double best = 0;
   pl->splits = 1;
   for (int s = 1; s <= pl->n_tiles && s <= 256; ++s) {
