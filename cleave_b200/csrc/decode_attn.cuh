@@ -50,8 +50,10 @@ enum DecodeMode { kPlain = 0, kWindow = 1, kWeights = 2, kSuffix = 3 };
 // The modes find the next piece and load its Q while the one before is merged, so a piece costs them less. 64 requests with
 // windows of 1004 tokens / 64 behind 8192 / 128 behind 32768: 53.7 / 45.7 / 192.0 us with 5, 52.9 / 45.2 / 190.6 with 3,
 // 52.9 / 45.5 / 197.0 with 2, 53.8 / 51.0 / 200.3 with 1.
-template <int MODE>
-constexpr int piece_units() { return MODE == kPlain ? kPieceUnits : 3; }
+// Where the tiles are no more than the CTAs, every tile is a CTA's whole share and nothing is left to balance: no units
+// then, so that the working CTAs are the first ones, which find SMs beside the prefix's
+// (4 requests behind 1000 tokens: 14.3 -> 11.3 us).
+constexpr int kPieceUnitsModes = 3;
 
 struct DecodeParams {
   const void* q;
@@ -68,6 +70,7 @@ struct DecodeParams {
   int batch, hkv, vblk, rows, page_size, num_pages, n_idx, kv_len, paged, box_tok;
   float scale_log2;
   int page_shift;  // log2 of page_size, or -1 where it is not a power of two
+  int piece_units; // modes: what starting and finishing a piece costs, in tiles
   // kWindow
   int window, sinks;
   // kWeights: scores, one row of raw_pitch floats per (request, query head); tokens beyond raw_len are not kept
@@ -187,6 +190,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nthreads = blockDim.x;
   const int hkvv = p.hkv * p.vblk;
+  const int w = MODE == kPlain ? kPieceUnits : p.piece_units;  // of a paged launch
 
   // The launch carries the programmatic-serialization attribute: this CTA may start while the kernel
   // before it in the stream is still draining. Nothing that kernel may have written (page tables, the
@@ -205,7 +209,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     for (int i = i0; i < i1; ++i) {
       const int n = item_valid_len(p, i);
       if (MODE != kPlain) V[i] = n;
-      sum += Walker::units(item_view<MODE, GATHER>(p, n).n_tiles(), piece_units<MODE>());
+      sum += Walker::units(item_view<MODE, GATHER>(p, n).n_tiles(), w);
     }
     scratch[tid] = sum;
     __syncthreads();
@@ -217,7 +221,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     int run = scratch[tid];
     for (int i = i0; i < i1; ++i) {
       P[i] = run;
-      run += Walker::units(item_view<MODE, GATHER>(p, MODE != kPlain ? V[i] : item_valid_len(p, i)).n_tiles(), piece_units<MODE>());
+      run += Walker::units(item_view<MODE, GATHER>(p, MODE != kPlain ? V[i] : item_valid_len(p, i)).n_tiles(), w);
     }
   } else {
     tiles_per_req = ceil_div(p.kv_len, kTile);
@@ -241,7 +245,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const int span = total > 0 ? ceil_div(total, G) : 1;
   const int u0 = min(static_cast<int>(blockIdx.x) * span, total);
   const int u1 = min(u0 + span, total);
-  Walker walker{p.paged ? P : nullptr, p.batch, hkvv, tiles_per_req, p.paged ? piece_units<MODE>() : 0};
+  Walker walker{p.paged ? P : nullptr, p.batch, hkvv, tiles_per_req, p.paged ? w : 0};
   if (!p.paged) {
     // Contiguous caches: where this CTA's first tiles lie follows from the launch parameters alone, so
     // while the preceding kernel still runs the TMA unit is asked to bring them into L2 (a hint: nothing
@@ -1054,6 +1058,7 @@ int plan_decode(const cb200_attn_decode_args* a, DecodeSetup* s, bool need_maps,
   s->partials_off = kWsHeaderBytes;
   s->counters_off = align_up(s->partials_off + static_cast<size_t>(sms) * 2 * kSlotBytesMax, 256);
   s->ws_needed = s->counters_off + static_cast<size_t>(a->batch) * p.hkv * p.vblk * 4;
+  p.piece_units = (tiles_ub - static_cast<long long>(a->batch) * kPieceUnits) * p.hkv * p.vblk <= grid ? 0 : kPieceUnitsModes;
   s->grid = static_cast<int>(units_ub < grid ? (units_ub > 0 ? units_ub : 1) : grid);
   if (!need_maps) return CB200_OK;
 

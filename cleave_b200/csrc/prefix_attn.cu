@@ -12,7 +12,7 @@
 // The prefix costs max(its bytes / bandwidth, 4 D flop per (query head, token) / tensor rate); up to 128 query rows per kv
 // head it is bound by the bytes, beyond that by the tensor cores and the exponentials.
 // Measured: 128 requests of 32 query and 8 kv heads of 128 over 32768 tokens 74 us (0.57 of the tensor rate; a tile takes
-// 1.15 us of an SM, most of it the latency of scores - softmax - value product), the whole with 1074 own tokens each 191 us.
+// 1.15 us of an SM, most of it the latency of scores - softmax - value product), the whole with 1074 own tokens each 189 us.
 //
 // The structure of the kernel (warp roles, tensor memory layout, lazy rescale) is that of attn_prefill_tc.cu with no mask
 // inside a tile but the prefix's end, keys from a page table, and partial results.
