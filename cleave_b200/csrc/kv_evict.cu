@@ -9,8 +9,8 @@
 // histograms over the sums, which it holds in registers, and writes the kept indices in order. evict_copy_kernel moves the
 // rows: it has no dependence between its CTAs (source and destination pages are disjoint), so it is a plain gather of
 // 2 D-byte rows that is bound by the memory's bandwidth, which is nearly all of the operator's time where the cache is large.
-// Measured: 32 requests of 1000 .. 8192 tokens cut to 2048, 8 heads of 128: 99 us (16 the selection, 83 the copy of 528 MB);
-// one request of 1500 cut to 512: 7.2 us.
+// Measured: 32 requests of 1000 .. 8192 tokens cut to 2048, 8 heads of 128: 92 us (the selection alone 16, the copy of 528
+// MB alone 83); one request of 1500 cut to 512: 6.7 us.
 
 #include "common.cuh"
 
@@ -34,7 +34,7 @@ struct EvictParams {
   int* kept;
   float* kept_sums;
   int* dst_last;
-  int hkv, row16, page_size, num_pages, n_idx, n_dst, max_len, budget, sinks, recent;  // row16: 16-byte chunks of a row
+  int batch, hkv, row16, page_size, num_pages, n_idx, n_dst, max_len, budget, sinks, recent;  // row16: 16-byte chunks of a row
 };
 
 // the range of a request in a page table that is caller data: clipped to the entries that exist
@@ -254,20 +254,26 @@ __global__ void __launch_bounds__(kSelThreads, KEYS <= 16 ? 2 : 1) evict_select_
   carry_sums();
 }
 
-// ROWS: (token, head) rows of K and of V per CTA
+// ROWS: (token, head) rows of K and of V per CTA.
+// The last and the first tokens of a request stay whatever their sums are: their rows come first in the grid, all requests'
+// before any other row, and are copied while the selection runs (it is latency bound and leaves the memory idle; 500 of 2048 tokens: 99 -> 92 us). The
+// selection lets this kernel start only once what precedes it is done, and writes nothing that is read before the wait.
 template <int ROWS>
 __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const EvictParams p) {
   __shared__ long long src_off[ROWS], dst_off[ROWS];  // in 16-byte chunks; dst < 0: no such page
-  pdl_wait();
-  const int b = blockIdx.y;
+  const int b = static_cast<int>(blockIdx.x) % p.batch;
   const Request r = request_of(p, b);
-  const long long rows = static_cast<long long>(r.keep) * p.hkv;  // (token, head), heads innermost
-  const long long r0 = static_cast<long long>(blockIdx.x) * ROWS;
-  if (r0 >= rows) return;
-  const int here = static_cast<int>(min(static_cast<long long>(ROWS), rows - r0));
+  const int first = min(p.sinks, r.keep), tail = min(p.recent, r.keep - first);
+  const long long rows = static_cast<long long>(r.keep) * p.hkv;  // (token, head), heads innermost; the last `tail` tokens in front
+  const long long r0 = static_cast<long long>(blockIdx.x / p.batch) * ROWS;
+  const int here = static_cast<int>(max(min(static_cast<long long>(ROWS), rows - r0), 0LL));
+  // the grid's last CTA always waits: the kernel must not be done before the selection is
+  if (r0 + here > static_cast<long long>(first + tail) * p.hkv || blockIdx.x == gridDim.x - 1) pdl_wait();
+  if (here == 0) return;
   for (int x = threadIdx.x; x < here; x += kCopyThreads) {
-    const int i = static_cast<int>((r0 + x) / p.hkv), h = static_cast<int>((r0 + x) % p.hkv);
-    const int j = __ldcg(p.kept + (static_cast<size_t>(b) * p.hkv + h) * p.budget + i);
+    const int t = static_cast<int>((r0 + x) / p.hkv), h = static_cast<int>((r0 + x) % p.hkv);
+    const int i = t < tail ? r.keep - tail + t : t - tail;
+    const int j = t < tail ? r.n - tail + t : i < first ? i : __ldcg(p.kept + (static_cast<size_t>(b) * p.hkv + h) * p.budget + i);
     const int sp = min(max(__ldg(p.kv_indices + r.src0 + j / p.page_size), 0), p.num_pages - 1);
     const int dp = __ldg(p.dst_indices + r.dst0 + i / p.page_size);
     src_off[x] = ((static_cast<long long>(sp) * p.page_size + j % p.page_size) * p.hkv + h) * p.row16;
@@ -318,7 +324,7 @@ extern "C" int cb200_kv_evict(const cb200_kv_evict_args* a, void* stream) {
   const long long rows = static_cast<long long>(a->budget) * a->num_kv_heads;
   const int copy_rows = rows * a->batch >= 128LL * 4 * 148 ? 128 : 32;
   const long long copy_ctas = (rows + copy_rows - 1) / copy_rows;
-  if (copy_ctas >= (1LL << 31)) return CB200_ERR_UNSUPPORTED;
+  if (copy_ctas * a->batch >= (1LL << 31)) return CB200_ERR_UNSUPPORTED;
   if (!a->k_cache || !a->v_cache || !a->weight_sums || !a->kv_indptr || !a->dst_indptr || !a->kept || !a->kept_sums || !a->dst_last_page_len)
     return CB200_ERR_BAD_ARG;
   if ((!a->kv_indices && a->num_kv_indices > 0) || (!a->dst_indices && a->num_dst_indices > 0)) return CB200_ERR_BAD_ARG;
@@ -336,6 +342,7 @@ extern "C" int cb200_kv_evict(const cb200_kv_evict_args* a, void* stream) {
   p.kept = a->kept;
   p.kept_sums = a->kept_sums;
   p.dst_last = a->dst_last_page_len;
+  p.batch = a->batch;
   p.hkv = a->num_kv_heads;
   p.row16 = a->head_dim / 8;
   p.page_size = a->page_size;
@@ -360,7 +367,7 @@ extern "C" int cb200_kv_evict(const cb200_kv_evict_args* a, void* stream) {
   const long long guess = longest < a->max_len ? longest : a->max_len;
   auto select = guess <= 4 * kSelThreads ? evict_select_kernel<4> : guess <= 16 * kSelThreads ? evict_select_kernel<16> : evict_select_kernel<kKeysMost>;
   CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, select, p));
-  cfg.gridDim = dim3(static_cast<unsigned>(copy_ctas), static_cast<unsigned>(a->batch), 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(copy_ctas * a->batch), 1, 1);
   cfg.blockDim = dim3(kCopyThreads, 1, 1);
   CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, copy_rows == 128 ? evict_copy_kernel<128> : evict_copy_kernel<32>, p));
   CB200_CUDA_TRY(cudaGetLastError());
