@@ -983,11 +983,16 @@ namespace {
 struct DecodeSetup {
   DecodeParams p;
   bool gather;
+  bool overlap;  // the launch may start while its predecessor drains; not for a caller that bounds the grid, see bounded()
   int grid, smem_bytes;
   size_t ws_needed, counters_off, partials_off;
   CUtensorMap tm_k, tm_v;
   GroupMaps tm_group;
 };
+
+// Whether max_ctas leaves less than the device. An operator of two kernels then keeps each of them to the bound and does not
+// let the second start beside the first.
+bool bounded(const cb200_attn_decode_args* a) { return a->max_ctas > 0 && a->max_ctas < sm_count(); }
 
 int plan_decode(const cb200_attn_decode_args* a, DecodeSetup* s, bool need_maps, bool modes = false) {
   if (!a) return CB200_ERR_BAD_ARG;
@@ -1060,6 +1065,7 @@ int plan_decode(const cb200_attn_decode_args* a, DecodeSetup* s, bool need_maps,
   s->ws_needed = s->counters_off + static_cast<size_t>(a->batch) * p.hkv * p.vblk * 4;
   p.piece_units = (tiles_ub - static_cast<long long>(a->batch) * kPieceUnits) * p.hkv * p.vblk <= grid ? 0 : kPieceUnitsModes;
   s->grid = static_cast<int>(units_ub < grid ? (units_ub > 0 ? units_ub : 1) : grid);
+  s->overlap = true;
   if (!need_maps) return CB200_OK;
 
   if (!a->q || !a->k_cache || !a->v_cache || !a->out) return CB200_ERR_BAD_ARG;
@@ -1134,7 +1140,7 @@ int launch_decode(const DecodeSetup& s, cudaStream_t stream) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = s.overlap ? 1 : 0;
   CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, s.tm_k, s.tm_v, s.tm_group, s.p));
   CB200_CUDA_TRY(cudaGetLastError());
   return CB200_OK;

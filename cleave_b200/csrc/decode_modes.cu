@@ -7,6 +7,8 @@
 
 #include "decode_attn.cuh"
 
+#include <algorithm>
+
 namespace cb200 {
 namespace {
 
@@ -17,11 +19,10 @@ namespace {
 // scores (written a moment ago, partly still in L2) and sums. A row whose scores are all -inf has no weights: it adds nothing.
 constexpr int kSumThreads = 256, kSumKeys = 4;
 
-__global__ void __launch_bounds__(kSumThreads) weight_sum_kernel(const DecodeParams p, float* __restrict__ sums) {
-  pdl_wait();
-  const int pair = blockIdx.y, b = pair / p.hkv;
+__device__ __forceinline__ void sum_block(const DecodeParams& p, float* __restrict__ sums, int pair, int block) {
+  const int b = pair / p.hkv;
   const int n = min(item_valid_len(p, b), p.raw_len);
-  const long long j0 = static_cast<long long>(blockIdx.x) * (kSumThreads * kSumKeys) + threadIdx.x;
+  const long long j0 = static_cast<long long>(block) * (kSumThreads * kSumKeys) + threadIdx.x;
   if (j0 >= n) return;
   const int j = static_cast<int>(j0), keys = min((n - j + kSumThreads - 1) / kSumThreads, kSumKeys);
   const size_t row = static_cast<size_t>(pair) * p.rows;
@@ -47,6 +48,13 @@ __global__ void __launch_bounds__(kSumThreads) weight_sum_kernel(const DecodePar
 #pragma unroll
   for (int i = 0; i < kSumKeys; ++i)
     if (i < keys) dst[i * kSumThreads] = old[i] + w[i];
+}
+
+// `blocks` blocks of keys for each of `pairs` (request, kv head); the grid has one CTA for each, or fewer of either
+__global__ void __launch_bounds__(kSumThreads) weight_sum_kernel(const DecodeParams p, float* __restrict__ sums, int blocks, int pairs) {
+  pdl_wait();
+  for (int pair = blockIdx.y; pair < pairs; pair += gridDim.y)
+    for (int block = blockIdx.x; block < blocks; block += gridDim.x) sum_block(p, sums, pair, block);
 }
 
 // floats between the score rows of two query heads: whole 32-byte runs
@@ -91,15 +99,21 @@ extern "C" int cb200_attn_decode_weights(const cb200_attn_decode_args* a, float*
   const int done = launch_decode_mode<kWeights>(s, a, st);
   if (done != CB200_OK) return done;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((max_len + static_cast<long long>(kSumKeys) * kSumThreads - 1) / (kSumKeys * kSumThreads)), static_cast<unsigned>(pairs), 1);
+  const int blocks = static_cast<int>((max_len + static_cast<long long>(kSumKeys) * kSumThreads - 1) / (kSumKeys * kSumThreads));
+  int grid_x = blocks, grid_y = static_cast<int>(pairs);
+  if (bounded(a)) {
+    grid_x = std::min(grid_x, a->max_ctas);
+    grid_y = std::min(grid_y, a->max_ctas / grid_x);
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>(grid_x), static_cast<unsigned>(grid_y), 1);
   cfg.blockDim = dim3(kSumThreads, 1, 1);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, weight_sum_kernel, s.p, weight_sums));
+  cfg.numAttrs = bounded(a) ? 0 : 1;
+  CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, weight_sum_kernel, s.p, weight_sums, blocks, static_cast<int>(pairs)));
   CB200_CUDA_TRY(cudaGetLastError());
   return CB200_OK;
 }

@@ -48,6 +48,7 @@ struct Params {
   float* ml;
   int* status;
   int len, page_size, num_pages, batch, hkv, group, per_block, blocks, splits, n_tiles;
+  int item0;  // the first of this launch's items
   float scale_log2;
 };
 
@@ -80,9 +81,10 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // row blocks of one part are neighbours: they read the same keys at the same time
-  const int blk = static_cast<int>(blockIdx.x) % p.blocks;
-  const int split = static_cast<int>(blockIdx.x) / p.blocks % p.splits;
-  const int h = static_cast<int>(blockIdx.x) / (p.blocks * p.splits);
+  const int item = p.item0 + static_cast<int>(blockIdx.x);
+  const int blk = item % p.blocks;
+  const int split = item / p.blocks % p.splits;
+  const int h = item / (p.blocks * p.splits);
   const int t0 = static_cast<int>(static_cast<long long>(p.n_tiles) * split / p.splits);
   const int nt = static_cast<int>(static_cast<long long>(p.n_tiles) * (split + 1) / p.splits) - t0;  // at least 1
 
@@ -423,8 +425,9 @@ int plan_prefix(const cb200_attn_decode_args* a, int prefix_len, Plan* pl) {
   pl->blocks = ceil_div(a->batch, pl->per_block);
   pl->n_tiles = static_cast<int>((static_cast<long long>(prefix_len) + kBN - 1) / kBN);
   const long long base = static_cast<long long>(a->num_kv_heads) * pl->blocks;
-  const int sms = sm_count();
+  int sms = sm_count();
   if (sms <= 0) return CB200_ERR_CUDA;
+  if (bounded(a)) sms = a->max_ctas;
   // Parts per (kv head, row block): the fewest rounds of tiles over the SMs, in units of a tile (about 1.2 us). A CTA
   // costs about three tiles beside its tiles (launch, first loads, the partial); every part adds one fp32 copy of
   // the rows that is written and read again, and every eight parts a round trip to L2 for each (request, kv head) of the
@@ -448,7 +451,7 @@ int plan_prefix(const cb200_attn_decode_args* a, int prefix_len, Plan* pl) {
 }
 
 template <typename T, int D, bool GATHER>
-int launch_prefix(const cb200_attn_decode_args* a, const Params& p, cudaStream_t stream) {
+int launch_prefix(const cb200_attn_decode_args* a, Params p, cudaStream_t stream) {
   const CUtensorMapDataType dt = a->dtype == CB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
   CUtensorMap tm_q, tm_k, tm_v;
@@ -473,7 +476,6 @@ int launch_prefix(const cb200_attn_decode_args* a, const Params& p, cudaStream_t
   auto kern = prefix_attn_kernel<T, D, GATHER>;
   CB200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmemBytes));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.hkv) * p.blocks * p.splits, 1, 1);
   cfg.blockDim = dim3(GATHER ? kThreadsGather : kThreads, 1, 1);
   cfg.dynamicSmemBytes = Cfg<D>::kSmemBytes;
   cfg.stream = stream;
@@ -482,7 +484,13 @@ int launch_prefix(const cb200_attn_decode_args* a, const Params& p, cudaStream_t
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm_q, tm_k, tm_v, p));
+  // One launch, or as many as keep each of them to the caller's bound; those behind the first wait for the one before
+  const int items = p.hkv * p.blocks * p.splits, most = bounded(a) ? std::min(items, a->max_ctas) : items;
+  for (p.item0 = 0; p.item0 < items; p.item0 += most) {
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min(most, items - p.item0)), 1, 1);
+    CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm_q, tm_k, tm_v, p));
+    cfg.numAttrs = 0;
+  }
   CB200_CUDA_TRY(cudaGetLastError());
   return CB200_OK;
 }
@@ -550,6 +558,7 @@ extern "C" int cb200_attn_decode_shared_prefix(const cb200_attn_decode_args* a, 
     s.p.pre_splits = pl.splits;
     s.p.pre_blocks = pl.blocks;
     s.p.pre_batch = pl.per_block;
+    s.overlap = !bounded(a);
   }
   return launch_decode_mode<kSuffix>(s, a, st);
 }

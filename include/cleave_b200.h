@@ -115,7 +115,8 @@ typedef struct {
   int32_t kv_len;         /* contiguous only: tokens per request */
   int32_t q_rows;         /* query rows per head (S_Q of the static operator); 0 or 1 = decode */
   int32_t dtype;          /* cb200_dtype */
-  int32_t max_ctas;       /* 0 = one CTA per SM; otherwise an upper bound on the grid */
+  int32_t max_ctas;       /* 0 = one CTA per SM; otherwise an upper bound on the grid: on each of them where an entry point
+                             launches several kernels, which then do not overlap */
   float sm_scale;
 } cb200_attn_decode_args;
 
