@@ -607,6 +607,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t s_col = lanes + kColS + g * 128, o_col = lanes + kColO + g * 128;
     const float scale = p.scale_log2;
+    constexpr float kHeadroom = weight_headroom<T>(kRescaleThreshold);  // P is at most 2^8
     const bool negative = scale < 0.f;  // the largest score is then the smallest product
     int n = 0, it = 0;  // tiles and items of this block so far
     Item w;
@@ -713,7 +714,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             }
           }
         }
-        const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+        const float m_use = m_ref == -INFINITY ? 0.f : m_ref - kHeadroom;
         if (!edge) {
           const uint64_t scale2 = pack_f32x2(scale, scale), shift2 = pack_f32x2(-m_use, -m_use);
           put_p(r[0], 0, scale2, shift2);
@@ -769,7 +770,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
 #pragma unroll 1
         for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + orow * D)[i] = make_uint4(0u, 0u, 0u, 0u);
       }
-      if (live_row && p.lse) p.lse[orow] = l_run > 0.f ? m_ref + fast_log2(l_run) : -INFINITY;
+      if (live_row && p.lse) p.lse[orow] = l_run > 0.f ? m_ref - kHeadroom + fast_log2(l_run) : -INFINITY;
     }
   }
 

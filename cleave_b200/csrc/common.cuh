@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/cleave_b200.h"
 
 namespace cb200 {
@@ -363,6 +365,16 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// Softmax weights P = 2^(x - m) are the 16-bit operand of the second product. fp16 holds numbers below 2^-14 in ever fewer
+// bits and none below 2^-25, and a row with one dominating key has all its others there. So P is scaled by
+// 2^headroom, whatever the bits above the largest P leave room for (`top`: log2 of that; 2^15 is fp16's last power of two). The
+// row sum carries the same factor: with m - headroom in the place of m, both come out as if m had been that. bf16 has the
+// exponents of fp32 and needs none.
+template <typename T>
+__host__ __device__ constexpr float weight_headroom(float top) {
+  return std::is_same<T, __half>::value ? 15.f - top : 0.f;
 }
 
 // What is left of (lo, hi) once they have been rounded to the 16-bit pair `rounded`, rounded itself: the pair and

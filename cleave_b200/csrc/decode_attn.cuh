@@ -24,9 +24,9 @@
 //   kSuffix   every request continues a prefix whose attention another kernel has left as fp32 partials (O, m, l):
 //             they are merged where the row's result is stored.
 // In these modes a token that takes no part adds nothing whatever its cache row holds (the plain mode multiplies
-// the rows behind a request's last token by zero), and P enters P V as the sum of two 16-bit numbers: the
-// warp MMAs have the room (the kernel is bound by the stream of K and V), and the error of the output is then
-// the rounding of the output alone.
+// the rows behind a request's last token by zero), and P enters P V as the sum of two 16-bit numbers, scaled where that keeps
+// them out of fp16's subnormal range: the warp MMAs have the room (the kernel is bound by the stream of K and V), and the
+// error of the output is then the rounding of the output alone.
 
 #pragma once
 
@@ -468,6 +468,8 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
   }
 
+  constexpr float kHeadroom = MODE == kPlain ? 0.f : weight_headroom<T>(0.f);  // P is at most 1
+
   const int ws = warp;  // token slice of this warp inside a tile
   const int r0 = lane >> 2, c2 = (lane & 3) * 2;
   const uint32_t stages_u32 = smem_u32(stages);
@@ -774,7 +776,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
               acc[n][3] *= sc1;
             }
           }
-          const float mu0 = m_run[0] == -INFINITY ? 0.f : m_run[0], mu1 = m_run[1] == -INFINITY ? 0.f : m_run[1];
+          const float mu0 = m_run[0] == -INFINITY ? 0.f : m_run[0] - kHeadroom, mu1 = m_run[1] == -INFINITY ? 0.f : m_run[1] - kHeadroom;
 #pragma unroll
           for (int u = 0; u < N; ++u) {
             // ---- P, as the sum of two 16-bit numbers
@@ -855,8 +857,8 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       *reinterpret_cast<float2*>(my_merge + (r0 + 8) * Plan::kMergePitch + n * 8 + c2) = make_float2(acc[n][2], acc[n][3]);
     }
     if ((lane & 3) == 0) {
-      my_merge[kRowsMax * Plan::kMergePitch + r0] = m_run[0];
-      my_merge[kRowsMax * Plan::kMergePitch + r0 + 8] = m_run[1];
+      my_merge[kRowsMax * Plan::kMergePitch + r0] = m_run[0] - kHeadroom;
+      my_merge[kRowsMax * Plan::kMergePitch + r0 + 8] = m_run[1] - kHeadroom;
       my_merge[kRowsMax * Plan::kMergePitch + kRowsMax + r0] = l_run[0];
       my_merge[kRowsMax * Plan::kMergePitch + kRowsMax + r0 + 8] = l_run[1];
     }

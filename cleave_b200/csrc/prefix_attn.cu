@@ -295,6 +295,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const int row = quarter * 32 + lane;  // query row of the block = tensor memory lane
     const uint32_t lane_field = static_cast<uint32_t>(quarter * 32) << 16;
     const int pair_bar = 1 + quarter;     // named barrier of the two warps that share the rows
+    constexpr float kHeadroom = weight_headroom<T>(kRescaleThreshold);  // P is at most 2^8
     float m_ref = 0.f, l_run = 0.f;
     for (int j = 0; j < nt; ++j) {
       const int sb = j & 1, pb = j & 1;
@@ -359,13 +360,14 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       }
       tc_fence_after();
       float psum = 0.f;
+      const float shift = m_ref - kHeadroom;
       {
         uint32_t pk[32];  // P in the storage type, as the operand of a 16-bit product must be; its sum is that of the fp32 values
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           const int c = 2 * i;
-          const float p0 = fast_exp2(__uint_as_float(r[c >> 5][c & 31]) - m_ref);
-          const float p1 = fast_exp2(__uint_as_float(r[(c + 1) >> 5][(c + 1) & 31]) - m_ref);
+          const float p0 = fast_exp2(__uint_as_float(r[c >> 5][c & 31]) - shift);
+          const float p1 = fast_exp2(__uint_as_float(r[(c + 1) >> 5][(c + 1) & 31]) - shift);
           psum += p0 + p1;
           pk[i] = pack2<T>(p0, p1);
         }
@@ -399,7 +401,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       }
     }
     if (!half && live_row) {
-      p.ml[part * 256 + row] = m_ref;
+      p.ml[part * 256 + row] = m_ref - kHeadroom;
       p.ml[part * 256 + kBM + row] = l_run + l_exch[row];
     }
   }
