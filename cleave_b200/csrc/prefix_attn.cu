@@ -296,7 +296,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const uint32_t lane_field = static_cast<uint32_t>(quarter * 32) << 16;
     const int pair_bar = 1 + quarter;     // named barrier of the two warps that share the rows
     constexpr float kHeadroom = weight_headroom<T>(kRescaleThreshold);  // P is at most 2^8
-    float m_ref = 0.f, l_run = 0.f;
+    float m_ref = -INFINITY, l_run = 0.f;  // m_ref is -inf until a score is not
     for (int j = 0; j < nt; ++j) {
       const int sb = j & 1, pb = j & 1;
       const int live = p.len - (t0 + j) * kBN - half * 64;  // scores of this thread's half that belong to the prefix
@@ -336,12 +336,10 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       mx = fmaxf(mx, mx_exch[(sb * 2 + (half ^ 1)) * kBM + row]);
       float alpha = 1.f;
       bool rescale = false;
-      if (j == 0) {
-        m_ref = mx == -INFINITY ? 0.f : mx;
-      } else if (mx > m_ref + kRescaleThreshold) {
+      if (mx > m_ref + kRescaleThreshold) {
         alpha = fast_exp2(m_ref - mx);
         m_ref = mx;
-        rescale = true;
+        rescale = j > 0;  // the first tile's product overwrites O
       }
       mbar_wait(&p_empty[pb], ((j >> 1) & 1) ^ 1, p.status, kFaultMmaBarrier);
       if (__any_sync(0xffffffffu, rescale)) {  // rare: the maximum grew by more than 2^8
@@ -353,14 +351,14 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           tmem_ld_32x32(tmem_base + lane_field + kColO + c0, o);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          for (int i = 0; i < 32; ++i) o[i] = alpha == 0.f ? 0u : __float_as_uint(__uint_as_float(o[i]) * alpha);
           tmem_st_32x32(tmem_base + lane_field + kColO + c0, o);
         }
         tmem_st_wait();
       }
       tc_fence_after();
       float psum = 0.f;
-      const float shift = m_ref - kHeadroom;
+      const float shift = m_ref == -INFINITY ? 0.f : m_ref - kHeadroom;
       {
         uint32_t pk[32];  // P in the storage type, as the operand of a 16-bit product must be; its sum is that of the fp32 values
 #pragma unroll

@@ -89,6 +89,27 @@ def test_growing_scores(page, big):
     c.check()
 
 
+def _low_scores(c, n, first):
+    """Keys whose scores are exact products, about -280 in log2 units; the first `first` of the prefix score -inf."""
+    c.q[...] = 0
+    c.q[..., 0] = 4.0
+    live = torch.arange(c.k[..., 0].numel()).view(c.k.shape[:-1]) % 8
+    c.k[..., 0] = -(384.0 + 2 * live).to(c.dtype)
+    for t in range(first):
+        c.k[c.pre_ids[t // c.page], t % c.page, :, 0] = -math.inf
+    c.before = tuple(x[c.pre_ids].flatten(0, 1)[:n] for x in (c.k, c.v))
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("max_ctas", [0, 1])  # every tile a part of its own; all of them one part
+@pytest.mark.parametrize("first", [128, 200, 300])
+def test_keys_of_weight_zero_in_front_of_low_scores(first, max_ctas, page):
+    """A part of the prefix, or its first tile, whose scores are all -inf holds nothing: no score of 0 that would outweigh the others."""
+    c = Case(300, [0, 70, 1], 4, 2, 64, page, torch.bfloat16, seed=11)
+    _low_scores(c, 300, first)
+    c.check(max_ctas=max_ctas)
+
+
 def test_more_prefix_pages_than_used():
     Case(130, [3, 70], 8, 2, 128, 64, torch.bfloat16, seed=7).check(extra_pages=4)
 
