@@ -737,7 +737,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         tc_fence_after();
         ++it;
       }
-      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+      const float inv = l_run != 0.f ? 1.f / l_run : 0.f;  // the sum of a row with a NaN score is NaN, and so is the row
       const bool aligned = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
       const size_t orow = static_cast<size_t>(w.q_base + row_of(w, g) + row) * p.hq + head_of(w, g);
 #pragma unroll 1
@@ -770,7 +770,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
 #pragma unroll 1
         for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + orow * D)[i] = make_uint4(0u, 0u, 0u, 0u);
       }
-      if (live_row && p.lse) p.lse[orow] = l_run > 0.f ? m_ref - kHeadroom + fast_log2(l_run) : -INFINITY;
+      if (live_row && p.lse) p.lse[orow] = l_run != 0.f ? m_ref - kHeadroom + fast_log2(l_run) : -INFINITY;
     }
   }
 

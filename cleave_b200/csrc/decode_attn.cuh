@@ -496,12 +496,13 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         Mf = Mn;
       }
     }
-    const float inv = Lf > 0.f ? 1.f / Lf : 0.f;
+    const bool some = MODE == kPlain ? Lf > 0.f : Lf != 0.f;  // modes: the sum of a row with a NaN score is NaN, and so is the row
+    const float inv = some ? 1.f / Lf : 0.f;
     T* dst = outp + row * D + mcol;
 #pragma unroll
     for (int k = 0; k < kQuads; ++k)
       *reinterpret_cast<uint2*>(dst + 32 * k) = make_uint2(pack2<T>(of[4 * k] * inv, of[4 * k + 1] * inv), pack2<T>(of[4 * k + 2] * inv, of[4 * k + 3] * inv));
-    if (p.lse && mcol == 0) p.lse[row] = Lf > 0.f ? Mf + fast_log2(Lf) : -INFINITY;
+    if (p.lse && mcol == 0) p.lse[row] = some ? Mf + fast_log2(Lf) : -INFINITY;
   };
   // kSuffix, all consumer threads: the partials of the prefix for an item's rows, summed into the merge buffer (rows of
   // O, then maxima and sums). A thread takes four columns of one row through all parts of the prefix, eight parts in
