@@ -19,7 +19,7 @@ namespace {
 // scores (written a moment ago, partly still in L2) and sums. A row whose scores are all -inf has no weights: it adds nothing.
 constexpr int kSumThreads = 256, kSumKeys = 4;
 
-__device__ __forceinline__ void sum_block(const DecodeParams& p, float* __restrict__ sums, int pair, int block) {
+__device__ __forceinline__ void sum_block(const DecodeParams& p, float* __restrict__ sums, int max_len, int pair, int block) {
   const int b = pair / p.hkv;
   const int n = min(item_valid_len(p, b), p.raw_len);
   const long long j0 = static_cast<long long>(block) * (kSumThreads * kSumKeys) + threadIdx.x;
@@ -28,7 +28,7 @@ __device__ __forceinline__ void sum_block(const DecodeParams& p, float* __restri
   const size_t row = static_cast<size_t>(pair) * p.rows;
   const float* x = p.raw + row * p.raw_pitch + j;
   const float* lse = p.lse + row;
-  float* dst = sums + static_cast<size_t>(pair) * p.raw_len + j;
+  float* dst = sums + static_cast<size_t>(pair) * max_len + j;
   float old[kSumKeys], w[kSumKeys];
 #pragma unroll
   for (int i = 0; i < kSumKeys; ++i) {
@@ -51,14 +51,20 @@ __device__ __forceinline__ void sum_block(const DecodeParams& p, float* __restri
 }
 
 // `blocks` blocks of keys for each of `pairs` (request, kv head); the grid has one CTA for each, or fewer of either
-__global__ void __launch_bounds__(kSumThreads) weight_sum_kernel(const DecodeParams p, float* __restrict__ sums, int blocks, int pairs) {
+__global__ void __launch_bounds__(kSumThreads) weight_sum_kernel(const DecodeParams p, float* __restrict__ sums, int max_len, int blocks, int pairs) {
   pdl_wait();
   for (int pair = blockIdx.y; pair < pairs; pair += gridDim.y)
-    for (int block = blockIdx.x; block < blocks; block += gridDim.x) sum_block(p, sums, pair, block);
+    for (int block = blockIdx.x; block < blocks; block += gridDim.x) sum_block(p, sums, max_len, pair, block);
 }
 
+// Tokens whose scores are kept: no request is longer than the page table, however wide the accumulators are (a server
+// that keeps room for its longest context would otherwise need scratch for that in every step).
+long long raw_tokens(const cb200_attn_decode_args* a, int max_len) {
+  const long long longest = static_cast<long long>(a->num_kv_indices) * a->page_size;
+  return longest < max_len ? longest : max_len;
+}
 // floats between the score rows of two query heads: whole 32-byte runs
-long long raw_pitch(int max_len) { return (static_cast<long long>(max_len) + 7) / 8 * 8; }
+long long raw_pitch(long long tokens) { return (tokens + 7) / 8 * 8; }
 
 }  // namespace
 }  // namespace cb200
@@ -76,8 +82,8 @@ extern "C" int cb200_attn_decode_window(const cb200_attn_decode_args* a, int win
 }
 
 extern "C" size_t cb200_attn_decode_weights_scratch_bytes(const cb200_attn_decode_args* a, int max_len) {
-  if (!a || a->batch <= 0 || a->num_qo_heads <= 0 || max_len <= 0) return 0;
-  return static_cast<size_t>(a->batch) * a->num_qo_heads * cb200::raw_pitch(max_len) * sizeof(float);
+  if (!a || a->batch <= 0 || a->num_qo_heads <= 0 || max_len <= 0 || a->num_kv_indices < 0 || a->page_size < 0) return 0;
+  return static_cast<size_t>(a->batch) * a->num_qo_heads * cb200::raw_pitch(cb200::raw_tokens(a, max_len)) * sizeof(float);
 }
 
 extern "C" int cb200_attn_decode_weights(const cb200_attn_decode_args* a, float* weight_sums, int max_len, void* scratch,
@@ -90,16 +96,18 @@ extern "C" int cb200_attn_decode_weights(const cb200_attn_decode_args* a, float*
   if (rc != CB200_OK) return rc;
   const long long pairs = static_cast<long long>(a->batch) * a->num_kv_heads;
   if (pairs > 65535) return CB200_ERR_UNSUPPORTED;
-  if (!scratch || scratch_bytes < cb200_attn_decode_weights_scratch_bytes(a, max_len)) return CB200_ERR_WORKSPACE;
+  const size_t need = cb200_attn_decode_weights_scratch_bytes(a, max_len);
+  if (need > 0 && (!scratch || scratch_bytes < need)) return CB200_ERR_WORKSPACE;
   if ((reinterpret_cast<uintptr_t>(scratch) & 31) || (reinterpret_cast<uintptr_t>(weight_sums) & 3)) return CB200_ERR_ALIGNMENT;
   s.p.raw = static_cast<float*>(scratch);
-  s.p.raw_len = max_len;
-  s.p.raw_pitch = raw_pitch(max_len);
+  const long long tokens = raw_tokens(a, max_len);
+  s.p.raw_len = static_cast<int>(tokens);
+  s.p.raw_pitch = raw_pitch(tokens);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int done = launch_decode_mode<kWeights>(s, a, st);
-  if (done != CB200_OK) return done;
+  if (done != CB200_OK || tokens == 0) return done;
   cudaLaunchConfig_t cfg = {};
-  const int blocks = static_cast<int>((max_len + static_cast<long long>(kSumKeys) * kSumThreads - 1) / (kSumKeys * kSumThreads));
+  const int blocks = static_cast<int>((tokens + kSumKeys * kSumThreads - 1) / (kSumKeys * kSumThreads));
   int grid_x = blocks, grid_y = static_cast<int>(pairs);
   if (bounded(a)) {
     grid_x = std::min(grid_x, a->max_ctas);
@@ -113,7 +121,7 @@ extern "C" int cb200_attn_decode_weights(const cb200_attn_decode_args* a, float*
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = bounded(a) ? 0 : 1;
-  CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, weight_sum_kernel, s.p, weight_sums, blocks, static_cast<int>(pairs)));
+  CB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, weight_sum_kernel, s.p, weight_sums, max_len, blocks, static_cast<int>(pairs)));
   CB200_CUDA_TRY(cudaGetLastError());
   return CB200_OK;
 }

@@ -268,8 +268,8 @@ def gqa_paged_decode_weights(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last
     (batch, HKV, max_len) is a contiguous fp32 tensor, updated in place; entries behind a request's last token stay as
     they are, and tokens from ``max_len`` on are attended but not recorded. Nothing is added with atomics: the sums are
     the same bits in every run, and requests may share pages. The scores of the step (4 bytes for every query head and
-    each of ``max_len`` tokens) are kept in scratch memory for the duration of the call. Returns ``(out, lse)``;
-    :func:`kv_cache_evict` reads the sums."""
+    each of ``max_len`` tokens, or of the whole page table's where they are fewer) are kept in scratch memory for the
+    duration of the call. Returns ``(out, lse)``; :func:`kv_cache_evict` reads the sums."""
     if _cuda(q, "q").device.index != torch.cuda.current_device():
         with torch.cuda.device(q.device):
             return gqa_paged_decode_weights(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale,

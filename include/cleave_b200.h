@@ -138,7 +138,8 @@ int cb200_attn_decode_window(const cb200_attn_decode_args* a, int window, int si
  * weight_sums is (batch, num_kv_heads, max_len), contiguous, updated in place; entries behind a
  * request's last token are left as they are, tokens from max_len on are attended but not recorded. Requests may share
  * pages. `lse` must not be NULL. `scratch` (cb200_attn_decode_weights_scratch_bytes, 32-byte aligned, any contents) holds
- * the scores between the two kernels. batch * num_kv_heads <= 65535. No counterpart in the reference.
+ * the scores between the two kernels: 4 bytes for each query head and each of min(max_len, num_kv_indices * page_size)
+ * tokens; it may be NULL where that is none. batch * num_kv_heads <= 65535. No counterpart in the reference.
  * ---------------------------------------------------------------------------------------- */
 size_t cb200_attn_decode_weights_scratch_bytes(const cb200_attn_decode_args* a, int max_len);
 int cb200_attn_decode_weights(const cb200_attn_decode_args* a, float* weight_sums, int max_len, void* scratch,

@@ -135,6 +135,24 @@ def test_weights_of_tokens_that_fit(max_len):
     _check_weights(Paged([0, 1, 300, 1999], 8, 2, 128, 64, torch.bfloat16, seed=30), max_len, steps=2)
 
 
+@pytest.mark.parametrize("lens", [[300, 41], [1], [0, 0], [64] * 5])
+def test_accumulators_wider_than_the_page_table(lens):
+    _check_weights(Paged(lens, 8, 2, 128, 16, torch.bfloat16, seed=34), 5003, steps=2)
+
+
+def test_wide_accumulators_need_no_scratch_of_their_width():
+    """Accumulators for 2^20 tokens over a page table of 320: the call's temporary memory follows the latter."""
+    ops, c = _ops(), Paged([300], 8, 2, 128, 64, torch.bfloat16, seed=35)
+    args, sums = c.args(), torch.zeros(1, 2, 1 << 20, device="cuda")
+    ops.gqa_paged_decode_weights(*args, sums)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.gqa_paged_decode_weights(*args, sums)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20
+    assert (sums[..., 300:] == 0).all()
+
+
 def test_weights_of_requests_that_share_pages():
     """Three requests over one page list: every one has sums of its own."""
     c = Paged([300], 8, 2, 128, 64, torch.float16, seed=31, q_rows=3)

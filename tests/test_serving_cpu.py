@@ -56,6 +56,17 @@ def test_decode_variants_refuse_their_own_arguments():
     assert L.cb200_attn_decode_shared_prefix(None, 4096, 1, 1, 4096, 4096, None) == BAD_ARG
 
 
+def test_scores_are_kept_for_no_more_tokens_than_the_page_table_holds():
+    f = _lib.lib().cb200_attn_decode_weights_scratch_bytes
+    bytes_of = lambda max_len, **kw: f(C.byref(_decode(**kw)), max_len)  # noqa: E731
+    assert bytes_of(131072) == bytes_of(128) == 2 * 8 * 128 * 4  # 8 pages of 16 tokens
+    assert bytes_of(127) == 2 * 8 * 128 * 4 and bytes_of(120) == 2 * 8 * 120 * 4
+    assert bytes_of(131072, num_kv_indices=3, page_size=5) == 2 * 8 * 16 * 4
+    assert bytes_of(131072, num_kv_indices=0) == 0
+    assert bytes_of(2 ** 31 - 1, num_kv_indices=2 ** 31 - 1) == 2 * 8 * 2 ** 31 * 4
+    assert bytes_of(100, num_kv_indices=-1) == 0
+
+
 def test_window_prefill_refuses_bad_arguments():
     def call(window=10, sinks=2, fill=0, **kw):
         a = _lib.AttnPrefillRaggedArgs()
