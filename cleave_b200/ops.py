@@ -159,6 +159,16 @@ def _check_all(device, **tensors) -> None:
             raise ValueError(f"{name} must be on {device}, not on {t.device}")
 
 
+_INT_MAX = 2 ** 31 - 1
+
+
+def _count(n: int, name: str) -> int:
+    """``n``, refused where the kernels' 32-bit arguments cannot hold it: it would be cut to another number."""
+    if n > _INT_MAX:
+        raise ValueError(f"{name} must be less than 2**31, got {n}")
+    return n
+
+
 def _empty2(rows, cols, device) -> torch.Tensor:
     """An uninitialised (rows, cols) float32 tensor (torch.empty takes a microsecond more to do the same)."""
     return torch.empty_strided((rows, cols), (cols, 1), dtype=torch.float32, device=device)
@@ -220,6 +230,7 @@ def _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page
         last = kv_last_page_len.data_ptr()
     elif page_size != 1:
         raise TypeError("missing input 'kv_last_page_len'")
+    n_idx = _count(kv_indices.numel(), "the entries of kv_indices")
     code = _dtype_code(q)
     if out is None:
         out = torch.empty_like(q)
@@ -230,7 +241,7 @@ def _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page
     elif tuple(lse.shape) != (batch, hq) or lse.dtype != torch.float32:
         raise ValueError("lse must be (batch, HQ) float32 on q's device")
     a = _lib.AttnDecodeArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), last,
-                            out.data_ptr(), lse.data_ptr(), None, 0, batch, hq, hkv, d, page_size, num_pages, kv_indices.numel(),
+                            out.data_ptr(), lse.data_ptr(), None, 0, batch, hq, hkv, d, page_size, num_pages, n_idx,
                             0, 1, code, max_ctas, sm_scale)
     return out, lse, a
 
@@ -239,8 +250,7 @@ def _window_args(window, sinks):
     window, sinks = int(window), int(sinks)
     if window < 1 or sinks < 0:
         raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
-    limit = 2 ** 31 - 1  # lengths are 32-bit counts: a larger window or number of sinks means all tokens
-    return min(window, limit), min(sinks, limit)
+    return min(window, _INT_MAX), min(sinks, _INT_MAX)  # lengths are 32-bit counts: more than that means all tokens
 
 
 def gqa_paged_decode_window(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, sm_scale, window, sinks=0, *,
@@ -280,7 +290,7 @@ def gqa_paged_decode_weights(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last
         raise TypeError("weight_sums must be float32")
     if weight_sums.dim() != 3 or tuple(weight_sums.shape[:2]) != (q.shape[0], k_cache.shape[2]):
         raise ValueError("weight_sums must be (batch, HKV, max_len)")
-    max_len = weight_sums.shape[2]
+    max_len = _count(weight_sums.shape[2], "max_len")
     L, stream = _lib.lib(), _raw_stream(q.device.index)
     need = L.cb200_attn_decode_weights_scratch_bytes(C.byref(a), max_len)
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
@@ -307,6 +317,7 @@ def gqa_paged_decode_shared_prefix(q, k_cache, v_cache, prefix_indices, prefix_l
         raise TypeError("prefix_indices must be int32")
     if prefix_len < 0 or prefix_len > prefix_indices.numel() * k_cache.shape[1]:
         raise ValueError(f"prefix_len must be between 0 and the {prefix_indices.numel()} pages of prefix_indices, got {prefix_len}")
+    _count(prefix_len, "prefix_len"), _count(prefix_indices.numel(), "the entries of prefix_indices")
     L, stream = _lib.lib(), _raw_stream(q.device.index)
     need = L.cb200_attn_decode_shared_prefix_scratch_bytes(C.byref(a), prefix_len)
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
@@ -328,6 +339,10 @@ def kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last
     source pages of this call nor used twice. Returns ``(kept, sums, last_page_len)``: the kept indices (batch, HKV,
     budget) int32, ascending, then -1; new accumulators (batch, HKV, max_len) that hold the kept tokens' sums, then 0; and
     (batch) int32, which with the destination tables is the shortened requests' page table."""
+    budget, sinks, recent = int(budget), int(sinks), int(recent)
+    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError(f"budget must be at least 1 and at least sinks + recent, got {budget}, {sinks} and {recent}")
+    _count(budget, "budget")
     if _cuda(k_cache, "k_cache").device.index != torch.cuda.current_device():
         with torch.cuda.device(k_cache.device):
             return kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last_page_len, dst_indptr, dst_indices,
@@ -335,9 +350,6 @@ def kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last
     device = k_cache.device
     _check_all(device, v_cache=v_cache, weight_sums=weight_sums, kv_indptr=kv_indptr, kv_indices=kv_indices,
                kv_last_page_len=kv_last_page_len, dst_indptr=dst_indptr, dst_indices=dst_indices)
-    budget, sinks, recent = int(budget), int(sinks), int(recent)
-    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
-        raise ValueError(f"budget must be at least 1 and at least sinks + recent, got {budget}, {sinks} and {recent}")
     _dtype_code(k_cache)
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
         raise ValueError("the caches must be (num_pages, page_size, HKV, D), of one storage dtype")
@@ -358,13 +370,15 @@ def kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last
         raise ValueError("kv_indptr and dst_indptr must have batch + 1 entries")
     if kv_last_page_len is not None and kv_last_page_len.numel() != batch:
         raise ValueError("kv_last_page_len must hold batch values")
+    n_idx, n_dst = _count(kv_indices.numel(), "the entries of kv_indices"), _count(dst_indices.numel(), "the entries of dst_indices")
+    _count(max_len, "max_len")
     kept = torch.empty_strided((batch, hkv, budget), (hkv * budget, budget, 1), dtype=i32, device=device)
     sums = torch.empty_like(weight_sums)
     last = torch.empty_strided((batch,), (1,), dtype=i32, device=device)
     a = _lib.KvEvictArgs(k_cache.data_ptr(), v_cache.data_ptr(), weight_sums.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(),
                          None if kv_last_page_len is None else kv_last_page_len.data_ptr(), dst_indptr.data_ptr(),
                          dst_indices.data_ptr(), kept.data_ptr(), sums.data_ptr(), last.data_ptr(), batch, hkv, d, page_size,
-                         num_pages, kv_indices.numel(), dst_indices.numel(), max_len, budget, sinks, recent)
+                         num_pages, n_idx, n_dst, max_len, budget, sinks, recent)
     _lib.check(_lib.lib().cb200_kv_evict(C.byref(a), _raw_stream(device.index)))
     return kept, sums, last
 
@@ -564,6 +578,7 @@ def gqa_paged_prefill(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_
 def _prefill_window(q, k, v, qo_indptr, kv_indptr, kv_indices, sm_scale, window, sinks, out, lse):
     device = q.device
     total_q, hq, d = q.shape
+    n_idx = 0 if kv_indices is None else _count(kv_indices.numel(), "the entries of kv_indices")
     fill = (1 if out is None else 0) | (2 if lse is None else 0)
     if out is None:
         out = torch.empty_like(q)
@@ -577,7 +592,7 @@ def _prefill_window(q, k, v, qo_indptr, kv_indptr, kv_indices, sm_scale, window,
     a = _lib.AttnPrefillRaggedArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), qo_indptr.data_ptr(), kv_indptr.data_ptr(),
                                    kv_indices.data_ptr() if paged else None, out.data_ptr(), lse.data_ptr(), None, 0,
                                    qo_indptr.numel() - 1, total_q, k.shape[0], hq, k.shape[-2], d, _dtype_code(q), 1, sm_scale,
-                                   kv_indices.numel() if paged else 0)
+                                   n_idx)
     L, stream = _lib.lib(), _raw_stream(device.index)
     _launch("attn_prefill", a, L.cb200_attn_prefill_ragged_workspace_bytes, device, stream,
             lambda: L.cb200_attn_prefill_ragged_window(C.byref(a), window, sinks, fill, stream))

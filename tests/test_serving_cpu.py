@@ -134,3 +134,10 @@ def test_windows_that_hold_nothing_are_refused(window, sinks):
     for fn, n in ((ops.gqa_paged_decode_window, 7), (ops.gqa_ragged_prefill_window, 6), (ops.gqa_paged_prefill_window, 7)):
         with pytest.raises(ValueError, match="window"):
             fn(*[None] * n, window, sinks)
+
+
+@pytest.mark.parametrize("budget", [0, -1, 2 ** 31, 2 ** 32 + 5, 2 ** 40])
+def test_budgets_that_hold_nothing_or_pass_32_bits_are_refused(budget):
+    """2 ** 32 + 5 would be cut to 5."""
+    with pytest.raises(ValueError, match="budget"):
+        ops.kv_cache_evict(*[None] * 8, budget=budget)

@@ -79,3 +79,28 @@ def test_prefill(paged):
         got = [ops.gqa_ragged_prefill_window(q, k[:, 0], v[:, 0], qp, _i32([0, shift, shift + 600]), 0.09, 100, 3)
                for (k, v), shift in ((small, 0), (large, base))]
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_counts_past_32_bits_are_refused():
+    """Tables and accumulators of 2 ** 32 + 4 entries, which a 32-bit count would take for 4. Nothing of them is read."""
+    from cleave_b200 import ops
+
+    (k, v), _, _ = _pools(64, 6)
+    q = torch.zeros(1, HQ, D, dtype=DT, device="cuda")
+    n = 2 ** 32 + 4
+    ptr, ids, last = _i32([0, 2]), _i32([0, 1]), _i32([64])
+    many = torch.empty(n, dtype=torch.int32, device="cuda")
+    sums = torch.zeros(1, HKV, 100, device="cuda")
+    bad = lambda fn, *a, **kw: pytest.raises(ValueError, fn, *a, **kw).match("2\\*\\*31")  # noqa: E731
+    bad(ops.gqa_paged_decode_window, q, k, v, ptr, many, last, 0.1, 10)
+    bad(ops.gqa_paged_decode_weights, q, k, v, ptr, many, last, 0.1, sums)
+    bad(ops.gqa_paged_decode_shared_prefix, q, k, v, many, 100, ptr, ids, last, 0.1)
+    bad(ops.gqa_paged_decode_shared_prefix, q, k, v, many[:2 ** 26 + 1], 2 ** 32 + 1, ptr, ids, last, 0.1)
+    bad(ops.kv_cache_evict, k, v, sums, ptr, many, last, ptr, ids, budget=8)
+    bad(ops.kv_cache_evict, k, v, sums, ptr, ids, last, ptr, many, budget=8)
+    bad(ops.gqa_paged_prefill_window, q, k.view(-1, 1, HKV, D), v.view(-1, 1, HKV, D), _i32([0, 1]), ptr, many, 0.1, 10)
+    del many
+    one_head = [torch.zeros(4, 64, 1, D, dtype=DT, device="cuda") for _ in range(2)]
+    wide = torch.empty(1, 1, n, device="cuda")
+    bad(ops.gqa_paged_decode_weights, q[:, :4].contiguous(), *one_head, ptr, ids, last, 0.1, wide)
+    bad(ops.kv_cache_evict, *one_head, wide, ptr, ids, last, ptr, _i32([2, 3]), budget=8)
