@@ -104,3 +104,31 @@ def test_counts_past_32_bits_are_refused():
     wide = torch.empty(1, 1, n, device="cuda")
     bad(ops.gqa_paged_decode_weights, q[:, :4].contiguous(), *one_head, ptr, ids, last, 0.1, wide)
     bad(ops.kv_cache_evict, *one_head, wide, ptr, ids, last, ptr, _i32([2, 3]), budget=8)
+
+
+@pytest.mark.parametrize("last", [2 ** 31 - 1, 17, -1, -2 ** 31])
+@pytest.mark.parametrize("op", ["plain", "window", "weights", "prefix", "evict"])
+def test_last_page_lengths_are_clipped_to_the_page(op, last):
+    """Whatever the table says about a last page, it holds between 0 and all of its 16 tokens; 2 ** 31 - 1 must not wrap to none."""
+    from cleave_b200 import ops
+
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(12, 16, 2, 64, generator=g).to(DT).cuda() for _ in range(2))
+    q, sums = torch.randn(2, 8, 64, generator=g).to(DT).cuda(), torch.rand(2, 2, 80, generator=g).cuda()
+    ptr, ids = _i32([0, 5, 7]), _i32([3, 0, 5, 1, 2, 4, 6])
+    got = []
+    for n in (last, min(max(last, 0), 16)):
+        table = (ptr, ids, _i32([n, 9]))
+        if op == "evict":
+            kk, vv = k.clone(), v.clone()
+            got.append((*ops.kv_cache_evict(kk, vv, sums, *table, _i32([0, 2, 4]), _i32([7, 8, 9, 10]), budget=30, sinks=2, recent=5), kk, vv))
+        elif op == "weights":
+            w = sums.clone()
+            got.append((*ops.gqa_paged_decode_weights(q, k, v, *table, 0.1, w), w))
+        elif op == "prefix":
+            got.append(ops.gqa_paged_decode_shared_prefix(q, k, v, ids, 30, *table, 0.1))
+        elif op == "window":
+            got.append(ops.gqa_paged_decode_window(q, k, v, *table, 0.1, 50, 2))
+        else:
+            got.append(ops.gqa_paged_decode(q, k, v, *table, 0.1))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
