@@ -116,6 +116,24 @@ def test_more_items_than_processors(paged):
 
 
 @PAGED
+@pytest.mark.parametrize("hq,hkv,d", [(12, 4, 64), (8, 8, 128), (10, 2, 64)])
+def test_more_items_than_processors_of_odd_groups(paged, hq, hkv, d):
+    """The blocks of an item are then two tiles of query rows, and the second exists in some items of a CTA and not in others."""
+    g = torch.Generator().manual_seed(13)
+    lens = []
+    for i in range(60):  # at most 128 rows, up to 256, and a little over 256
+        n = int(torch.randint(1, 129, (1,), generator=g)) + (0, 128, 256)[i % 3]
+        lens.append((n, n + int(torch.randint(0, 200, (1,), generator=g))))
+    Case(lens, hq, hkv, d, torch.bfloat16, 140, 2, paged, seed=14).check()
+
+
+@PAGED
+@pytest.mark.parametrize("hq,hkv,d", [(12, 4, 128), (8, 8, 64), (10, 2, 128)])
+def test_long_prompts_persistent_of_odd_groups(paged, hq, hkv, d):
+    Case([(2500, 2600), (100, 900), (1, 1), (3000, 3000)], hq, hkv, d, torch.float16, 700, 4, paged, seed=15).check()
+
+
+@PAGED
 def test_long_prompt_persistent(paged):
     Case([(2500, 2600)], 16, 4, 128, torch.bfloat16, 700, 4, paged, seed=5).check()
 
