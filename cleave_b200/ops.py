@@ -14,6 +14,7 @@ from . import _lib
 
 _DT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _workspaces: dict = {}
+_outgrown: list = []  # workspaces that a larger one has replaced
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -45,6 +46,11 @@ def workspace(kind: str, nbytes: int, device) -> torch.Tensor:
     key = (kind, index, _stream())
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
+        if ws is not None:
+            # A graph that was captured on this stream may hold the old one's address and is replayed after this. Growing
+            # to twice the size at least keeps all of the old ones together below the size of the new one.
+            _outgrown.append(ws)
+            nbytes = max(nbytes, 2 * ws.numel())
         ws = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)  # never smaller than the status header
         _workspaces[key] = ws
     return ws
