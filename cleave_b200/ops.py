@@ -45,6 +45,11 @@ def workspace(kind: str, nbytes: int, device) -> torch.Tensor:
         index = torch.cuda.current_device()
     key = (kind, index, _stream())
     ws = _workspaces.get(key)
+    if (ws is None or ws.numel() < nbytes) and torch.cuda.is_current_stream_capturing():
+        # What is allocated now comes from the graph's pool and is zero only once the graph has run: captures may share
+        # it, calls outside of them must not find it
+        key = (*key, "captured")
+        ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
         if ws is not None:
             # A graph that was captured on this stream may hold the old one's address and is replayed after this. Growing

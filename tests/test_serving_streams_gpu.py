@@ -66,3 +66,27 @@ def test_two_streams_at_once(op):
         for i in range(2):
             for r in got[i]:
                 assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+def test_eager_calls_after_a_capture_on_their_stream(monkeypatch):
+    """A graph of the plain decode is captured on a fresh stream and not replayed: what it allocated holds anything."""
+    from cleave_b200 import ops
+
+    c = Paged([900, 33, 500], 8, 2, 128, 16, torch.bfloat16, seed=3)
+    c.k.nan_to_num_(0.0), c.v.nan_to_num_(0.0)
+    args = c.args()
+    want, plain = ops.gqa_paged_decode_window(*args, 300, 4), ops.gqa_paged_decode(*args)
+    torch.cuda.synchronize()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    monkeypatch.setattr(ops, "_workspaces", {})
+    with torch.cuda.graph(graph, stream=stream):
+        held = ops.gqa_paged_decode(*args)
+    with torch.cuda.stream(stream):
+        got = ops.gqa_paged_decode_window(*args, 300, 4)
+    torch.cuda.synchronize()
+    assert len(ops._workspaces) == 2
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(held, plain))

@@ -43,3 +43,18 @@ def test_outgrown_workspaces_are_smaller_than_the_one_in_use(host):
     for n in range(1000, 100000, 777):
         ws = ops.workspace("a", n, "cpu")
     assert sum(t.numel() for t in ops._outgrown) < ws.numel() < 2 * 100000
+
+
+def test_a_workspace_made_under_capture_stays_with_captures(host):
+    """It lies in the graph's pool and is zero-filled by the graph alone, when that is replayed."""
+    host["capturing"] = True
+    captured = ops.workspace("a", 1000, "cpu")
+    assert ops.workspace("a", 1000, "cpu") is captured
+    host["capturing"] = False
+    eager = ops.workspace("a", 1000, "cpu")
+    assert eager is not captured
+    host["capturing"] = True
+    assert ops.workspace("a", 1000, "cpu") is eager  # one that is zero already serves a capture too
+    larger = ops.workspace("a", 5000, "cpu")
+    host["capturing"] = False
+    assert ops.workspace("a", 1000, "cpu") is eager and ops.workspace("a", 5000, "cpu") is not larger
