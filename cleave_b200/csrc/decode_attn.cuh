@@ -120,8 +120,10 @@ __device__ __forceinline__ int item_valid_len(const DecodeParams& p, int b) {
   if (!p.paged) return p.kv_len;
   const int n_pages = item_pages(p, b);
   if (p.page_size == 1 || p.kv_last == nullptr) return n_pages * p.page_size;
-  // the count is caller data: clipped before it is added, so that the sum stays in 32 bits
-  return n_pages > 0 ? (n_pages - 1) * p.page_size + min(max(p.kv_last[b], 0), p.page_size) : 0;
+  // the count is caller data: clipped before it is added, so that the sum stays in 32 bits (and loaded whatever n_pages is, so
+  // that the load does not wait for the page table's)
+  const int v = max(n_pages - 1, 0) * p.page_size + min(max(p.kv_last[b], 0), p.page_size);
+  return min(v, n_pages * p.page_size);
 }
 
 // The tiles of a request with n tokens that are in the stream. Whole boxes of the cache (TMA): tile t of the item is tile t

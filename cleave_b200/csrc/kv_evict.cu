@@ -56,7 +56,7 @@ __device__ __forceinline__ Request request_of(const EvictParams& p, int b) {
   if (p.page_size == 1 || p.kv_last == nullptr) {
     r.n = src.y * p.page_size;
   } else {
-    r.n = src.y > 0 ? (src.y - 1) * p.page_size + min(max(p.kv_last[b], 0), p.page_size) : 0;
+    r.n = min(max(src.y - 1, 0) * p.page_size + min(max(p.kv_last[b], 0), p.page_size), src.y * p.page_size);
   }
   const long long room = static_cast<long long>(dst.y) * p.page_size;
   r.keep = static_cast<int>(min(static_cast<long long>(min(r.n, p.budget)), room));
