@@ -173,11 +173,9 @@ def _check_all(device, **tensors) -> None:
 _INT_MAX = 2 ** 31 - 1
 
 
-def _count(n: int, name: str) -> int:
-    """``n``, refused where the kernels' 32-bit arguments cannot hold it: it would be cut to another number."""
-    if n > _INT_MAX:
-        raise ValueError(f"{name} must be less than 2**31, got {n}")
-    return n
+def _too_many(name: str, n: int) -> None:
+    """A count that the kernels' 32-bit arguments cannot hold: it would be cut to another number."""
+    raise ValueError(f"{name} must be less than 2**31, got {n}")
 
 
 def _empty2(rows, cols, device) -> torch.Tensor:
@@ -241,7 +239,9 @@ def _paged_decode_setup(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page
         last = kv_last_page_len.data_ptr()
     elif page_size != 1:
         raise TypeError("missing input 'kv_last_page_len'")
-    n_idx = _count(kv_indices.numel(), "the entries of kv_indices")
+    n_idx = kv_indices.numel()
+    if n_idx > _INT_MAX:
+        _too_many("the entries of kv_indices", n_idx)
     code = _dtype_code(q)
     if out is None:
         out = torch.empty_like(q)
@@ -301,7 +301,9 @@ def gqa_paged_decode_weights(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last
         raise TypeError("weight_sums must be float32")
     if weight_sums.dim() != 3 or tuple(weight_sums.shape[:2]) != (q.shape[0], k_cache.shape[2]):
         raise ValueError("weight_sums must be (batch, HKV, max_len)")
-    max_len = _count(weight_sums.shape[2], "max_len")
+    max_len = weight_sums.shape[2]
+    if max_len > _INT_MAX:
+        _too_many("max_len", max_len)
     L, stream = _lib.lib(), _raw_stream(q.device.index)
     need = L.cb200_attn_decode_weights_scratch_bytes(C.byref(a), max_len)
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
@@ -328,12 +330,14 @@ def gqa_paged_decode_shared_prefix(q, k_cache, v_cache, prefix_indices, prefix_l
         raise TypeError("prefix_indices must be int32")
     if prefix_len < 0 or prefix_len > prefix_indices.numel() * k_cache.shape[1]:
         raise ValueError(f"prefix_len must be between 0 and the {prefix_indices.numel()} pages of prefix_indices, got {prefix_len}")
-    _count(prefix_len, "prefix_len"), _count(prefix_indices.numel(), "the entries of prefix_indices")
+    n_pre = prefix_indices.numel()
+    if n_pre > _INT_MAX or prefix_len > _INT_MAX:
+        _too_many("prefix_len and the entries of prefix_indices", max(n_pre, prefix_len))
     L, stream = _lib.lib(), _raw_stream(q.device.index)
     need = L.cb200_attn_decode_shared_prefix_scratch_bytes(C.byref(a), prefix_len)
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
     _launch("attn_decode", a, L.cb200_attn_decode_workspace_bytes, q.device, stream,
-            lambda: L.cb200_attn_decode_shared_prefix(C.byref(a), prefix_indices.data_ptr(), prefix_indices.numel(), prefix_len,
+            lambda: L.cb200_attn_decode_shared_prefix(C.byref(a), prefix_indices.data_ptr(), n_pre, prefix_len,
                                                       scratch.data_ptr(), need, stream))
     return out, lse
 
@@ -353,7 +357,8 @@ def kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last
     budget, sinks, recent = int(budget), int(sinks), int(recent)
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"budget must be at least 1 and at least sinks + recent, got {budget}, {sinks} and {recent}")
-    _count(budget, "budget")
+    if budget > _INT_MAX:
+        _too_many("budget", budget)
     if _cuda(k_cache, "k_cache").device.index != torch.cuda.current_device():
         with torch.cuda.device(k_cache.device):
             return kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last_page_len, dst_indptr, dst_indices,
@@ -381,8 +386,9 @@ def kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last
         raise ValueError("kv_indptr and dst_indptr must have batch + 1 entries")
     if kv_last_page_len is not None and kv_last_page_len.numel() != batch:
         raise ValueError("kv_last_page_len must hold batch values")
-    n_idx, n_dst = _count(kv_indices.numel(), "the entries of kv_indices"), _count(dst_indices.numel(), "the entries of dst_indices")
-    _count(max_len, "max_len")
+    n_idx, n_dst = kv_indices.numel(), dst_indices.numel()
+    if n_idx > _INT_MAX or n_dst > _INT_MAX or max_len > _INT_MAX:
+        _too_many("max_len and the entries of kv_indices and dst_indices", max(n_idx, n_dst, max_len))
     kept = torch.empty_strided((batch, hkv, budget), (hkv * budget, budget, 1), dtype=i32, device=device)
     sums = torch.empty_like(weight_sums)
     last = torch.empty_strided((batch,), (1,), dtype=i32, device=device)
@@ -589,7 +595,9 @@ def gqa_paged_prefill(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_
 def _prefill_window(q, k, v, qo_indptr, kv_indptr, kv_indices, sm_scale, window, sinks, out, lse):
     device = q.device
     total_q, hq, d = q.shape
-    n_idx = 0 if kv_indices is None else _count(kv_indices.numel(), "the entries of kv_indices")
+    n_idx = 0 if kv_indices is None else kv_indices.numel()
+    if n_idx > _INT_MAX:
+        _too_many("the entries of kv_indices", n_idx)
     fill = (1 if out is None else 0) | (2 if lse is None else 0)
     if out is None:
         out = torch.empty_like(q)
