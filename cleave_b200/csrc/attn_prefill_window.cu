@@ -11,7 +11,8 @@
 // Why two: one block is a chain - scores, softmax, value product - in which the tensor cores idle during the softmax and
 // the softmax warps during the products. With two blocks in turn the one's softmax runs beside the other's products, and a
 // CTA asks L2 for half as many keys per row. Measured for one prompt of 8191 tokens, window 1024, 32/8 heads of 128:
-// 206 us where the same tiles on the one-block kernel of the plain prefill take 232; a step of both blocks takes 4200
+// 206 .. 208 us where the same tiles on the one-block kernel of the plain prefill take 232 (five chunks of 1 .. 130 rows, where most
+// items are one short chain and half of the SMs have none, take 25 where one block an item took 22: one kernel serves both); a step of both blocks takes 4200
 // cycles, of which the tensor cores work 2050 and the exponentials' unit as much. What remains is latency: a softmax warp
 // has its scheduler nearly to itself while the other block's products run, and issues an exponential every 16
 // cycles where two warps at work issue one every 9.
@@ -23,7 +24,7 @@
 // keys are gathered row by row, copy K and V.
 // The softmax keeps a reference maximum per row and rescales O (in tensor memory) only when the maximum has grown by
 // more than 2^8; the factor is applied to O and to the row sum alike. P is rounded to the storage type, as the operand of
-// a 16-bit product must be; everything else is held in 32 bits.
+// a 16-bit product must be, and in fp16 scaled by 2^7 before (weight_headroom); everything else is held in 32 bits.
 // CTAs are persistent: one per SM, items from a counter in the workspace header that clears itself.
 // Keys that no row of an item sees (behind the last row, between the sinks and the window) add nothing whatever their
 // rows hold: their scores are masked, and their rows of V are zero.

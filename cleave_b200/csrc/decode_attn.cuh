@@ -50,9 +50,10 @@ enum DecodeMode { kPlain = 0, kWindow = 1, kWeights = 2, kSuffix = 3 };
 // The modes find the next piece and load its Q while the one before is merged, so a piece costs them less. 64 requests with
 // windows of 1004 tokens / 64 behind 8192 / 128 behind 32768: 53.7 / 45.7 / 192.0 us with 5, 52.9 / 45.2 / 190.6 with 3,
 // 52.9 / 45.5 / 197.0 with 2, 53.8 / 51.0 / 200.3 with 1.
-// Where the tiles are no more than the CTAs, every tile is a CTA's whole share and nothing is left to balance: no units
-// then, so that the working CTAs are the first ones, which find SMs beside the prefix's
-// (4 requests behind 1000 tokens: 14.3 -> 11.3 us).
+// Three shapes are what this constant rests on. Where the page table has no more tiles than there are CTAs, every tile is a
+// CTA's whole share and nothing is left to balance: no units then, so that the working CTAs are the first ones, which find SMs
+// beside the prefix's (4 requests behind 1000 tokens: 14.3 -> 11.3 us). The rule knows the table, not the stream: a short
+// window over a long table keeps the units although its tiles are few.
 constexpr int kPieceUnitsModes = 3;
 
 struct DecodeParams {
@@ -79,7 +80,7 @@ struct DecodeParams {
   long long raw_pitch;
   // kSuffix: partials of the prefix, pre_splits of them per (kv head, block of 128 query rows), see prefix_attn.cu
   const float* pre_o;   // [kv head][row block][split][128][D], relative to the split's reference maximum
-  const float* pre_ml;  // [kv head][row block][split][2][128]: reference maximum (log2 units), sum
+  const float* pre_ml;  // [kv head][row block][split][2][128]: reference maximum (log2 units; -inf: no score is finite), sum
   int pre_splits, pre_blocks, pre_batch;  // pre_batch: requests per row block
 };
 

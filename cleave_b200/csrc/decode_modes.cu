@@ -1,9 +1,9 @@
 // Decode attention over a sliding window with sinks, and decode that accumulates attention weights: entry points
 // over the modes of the kernel in decode_attn.cuh, and the kernel that turns kept scores into weights.
 //
-// Measured (32 query and 8 kv heads of 128, graph replays): windows of 1004 tokens, 64 requests, 16-token pages 53.0 us, 4.9 TB/s;
-// windows of 4160, 128 requests, 64-token pages 332 us, 6.1 TB/s; weights of 64 requests of 512 .. 8192 tokens, 16-token pages
-// 224 .. 228 us, of which the second kernel takes 15.
+// Measured (32 query and 8 kv heads of 128, graph replays): windows of 1004 tokens, 64 requests, 16-token pages 52.8 us, 4.9 TB/s;
+// windows of 4160, 128 requests, 64-token pages 333 us, 6.1 TB/s; weights of 64 requests of 512 .. 8192 tokens, 16-token pages
+// 224 .. 229 us, of which the second kernel takes 15.
 
 #include "decode_attn.cuh"
 

@@ -6,13 +6,14 @@
 //   1. prefix_attn_kernel, here: the query rows of all requests that read one kv head (batch * HQ / HKV rows) attend the
 //      prefix as ONE problem on the tcgen05 tensor cores. An item is (kv head, block of 128 query rows, part of the
 //      prefix's tiles of 128 tokens); the prefix is cut into as many parts as fill the SMs. Each item leaves fp32
-//      (O, m, l) in the scratch buffer.
+//      (O, m, l) in the scratch buffer. P is one 16-bit operand here, in fp16 scaled by 2^7 (weight_headroom), so this
+//      kernel sets the error of the result: the two-part P of the second one helps where a request's own tokens weigh most.
 //   2. decode_attn_kernel in its suffix mode: the stream over the requests' own tokens; where a row's result is
 //      stored, the row's prefix parts are merged in. No third launch, and the requests' own part may be empty.
 // The prefix costs max(its bytes / bandwidth, 4 D flop per (query head, token) / tensor rate); up to 128 query rows per kv
 // head it is bound by the bytes, beyond that by the tensor cores and the exponentials.
 // Measured: 128 requests of 32 query and 8 kv heads of 128 over 32768 tokens 74 us (0.57 of the tensor rate; a tile takes
-// 1.15 us of an SM, most of it the latency of scores - softmax - value product), the whole with 1074 own tokens each 189 us.
+// 1.15 us of an SM, most of it the latency of scores - softmax - value product), the whole with 1074 own tokens each 188 us.
 //
 // The structure of the kernel (warp roles, tensor memory layout, lazy rescale) is that of attn_prefill_tc.cu with no mask
 // inside a tile but the prefix's end, keys from a page table, and partial results.

@@ -318,7 +318,8 @@ def gqa_paged_decode_shared_prefix(q, k_cache, v_cache, prefix_indices, prefix_l
     the pages ``prefix_indices`` (int32), then its own tokens, which ``kv_indptr`` / ``kv_indices`` / ``kv_last_page_len``
     describe as usual (a request may have none). The prefix's rows are read once for the batch, not once per request.
     ``prefix_len`` is a number; only the first ``ceil(prefix_len / page_size)`` entries of ``prefix_indices`` are used. At
-    most 128 query heads per kv head. Returns ``(out, lse)`` over both parts, ``lse`` base 2."""
+    most 128 query heads per kv head. ``max_ctas`` bounds the grids of both kernels, which then run one after the other.
+    Returns ``(out, lse)`` over both parts, ``lse`` base 2."""
     if _cuda(q, "q").device.index != torch.cuda.current_device():
         with torch.cuda.device(q.device):
             return gqa_paged_decode_shared_prefix(q, k_cache, v_cache, prefix_indices, prefix_len, kv_indptr, kv_indices,
@@ -351,7 +352,8 @@ def kv_cache_evict(k_cache, v_cache, weight_sums, kv_indptr, kv_indices, kv_last
     ``weight_sums`` (batch, HKV, max_len) fp32; ``kv_indptr`` and ``dst_indptr`` (batch + 1) int32 in pages. Give a
     request of ``n`` tokens ``ceil(min(n, budget) / page_size)`` destination pages (with fewer, fewer tokens stay).
     Source pages are only read and may be shared; destination pages must be pages of the same pool that are neither
-    source pages of this call nor used twice. Returns ``(kept, sums, last_page_len)``: the kept indices (batch, HKV,
+    source pages of this call nor used twice. Sums come from decode steps alone: after a prefill all are equal, and an
+    eviction then keeps the first tokens beside the sinks and the recent ones. Returns ``(kept, sums, last_page_len)``: the kept indices (batch, HKV,
     budget) int32, ascending, then -1; new accumulators (batch, HKV, max_len) that hold the kept tokens' sums, then 0; and
     (batch) int32, which with the destination tables is the shortened requests' page table."""
     budget, sinks, recent = int(budget), int(sinks), int(recent)
